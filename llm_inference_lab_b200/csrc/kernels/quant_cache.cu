@@ -1,0 +1,346 @@
+// A paged cache in 8 bits (quant8.cuh): keys rotated, keys and values rounded and written to their pages, and rows of such
+// pages read back.
+//
+//   store   q' = q turned by its row's angles, rounded to the storage type; k' = k turned, v: to codes and a byte a row
+//           (lo, hi) -> (lo c - hi s, hi c + lo s), elements i and i + rotary_dim / 2 of a head; c, s from the step's table
+//   load    code * 2^(e - 127)
+//
+// A key's code is the one nearest to the exact k': the products of 8- or 24-bit numbers with the table's are formed in 64 bits,
+// and one rounding leads from there to 8 bits (a product rounded to 32 bits, let alone to 16, before its code is chosen takes
+// the neighbouring code now and then).  So the cache depends on the inputs alone, not on the order of anything.  Queries are turned in 32
+// bits as everywhere (rowwise.cu): their result is rounded once.
+//
+// Both are bound by memory: a row's lanes hold it in registers between the one read and the one write, and the row's largest
+// magnitude goes around its lanes by shuffles.
+#include "quant8.cuh"
+
+namespace {
+
+constexpr int THREADS = 256, FEW_THREADS = 64;
+constexpr int MOST_DIM = 256;
+
+struct Store {
+  const void* rows;          // [tokens, row_stride] of T, or [parts, tokens, width] floats
+  long long row_stride;
+  int parts;                 // 0: rows of T
+  long long part_stride;
+  const __nv_bfloat16* bias; // [width] or null (parts only)
+  const float2* table;       // [tokens, rotary_dim / 2] (cos, sin), null with rotary_dim 0
+  int rotary_dim;
+  const int* slots;          // [tokens], negative: not stored
+  void* q_out;               // [tokens, n_q * d] of T
+  uint8_t *k, *v, *k_scale, *v_scale;
+  int tokens, n_q, n_kv, d, page_size, num_pages;
+};
+
+// Where a row of the cache lies: its number among the pool's rows, or -1.
+__device__ __forceinline__ long long pool_row(const Store& s, int token, int kv_head, bool reports) {
+  const int slot = s.slots[token];
+  if (slot < 0) return -1;
+  const int page = slot / s.page_size;
+  if (page >= s.num_pages) {
+    if (reports) lab_set_error(LAB_ERR_PAGE_RANGE);
+    return -1;
+  }
+  return ((long long)page * s.n_kv + kv_head) * s.page_size + (slot - page * s.page_size);
+}
+
+// N neighbouring numbers of a row.  PARTS: the parts are summed in 64 bits in their order, the bias added, and the sum rounded
+// once to bfloat16, the type that the rows would have.
+template <typename T, bool PARTS, int N>
+__device__ __forceinline__ void take(const Store& s, int token, int col, float (&x)[N]) {
+  if constexpr (PARTS) {
+    const float* p = static_cast<const float*>(s.rows) + (size_t)token * s.row_stride + col;
+    double sum[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = 0.0;
+    for (int s0 = 0; s0 < s.parts; s0 += 8) {      // eight loads in flight
+      float f[8][N];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[i][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < s.parts) {
+          if constexpr (N == 2) {
+            const float2 w = *reinterpret_cast<const float2*>(p + (s0 + i) * s.part_stride);
+            f[i][0] = w.x, f[i][1] = w.y;
+          } else {
+            f[i][0] = p[(s0 + i) * s.part_stride];
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] += f[i][j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (s.bias) sum[j] += to_f32(s.bias[col + j]);
+      x[j] = round_to<__nv_bfloat16>(q8_to_odd(sum[j]));
+    }
+  } else {
+    const T* p = static_cast<const T*>(s.rows) + (size_t)token * s.row_stride + col;
+    if constexpr (N == 8) {
+      const float4 a = load4(p), b = load4(p + 4);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = to_f32(p[j]);
+    }
+  }
+}
+// 16 bytes a load where the row's bytes allow it: bfloat16 rows, eight at a time.
+template <>
+__device__ __forceinline__ void take<__nv_bfloat16, false, 8>(const Store& s, int token, int col, float (&x)[8]) {
+  const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(s.rows) + (size_t)token * s.row_stride + col);
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+}
+
+template <int N> __device__ __forceinline__ void put(__nv_bfloat16* to, const float (&x)[N]) {
+  if constexpr (N == 8)
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  else
+    *reinterpret_cast<uint32_t*>(to) = pack_bf16(x[0], x[1]);
+}
+template <int N> __device__ __forceinline__ void put(float* to, const float (&x)[N]) {
+  if constexpr (N == 8) {
+    store4(to, make_float4(x[0], x[1], x[2], x[3]));
+    store4(to + 4, make_float4(x[4], x[5], x[6], x[7]));
+  } else {
+    *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+  }
+}
+template <int N> __device__ __forceinline__ void put_codes(uint8_t* to, const float (&x)[N], float inverse) {
+  if constexpr (N == 8)
+    *reinterpret_cast<uint2*>(to) = make_uint2(q8_encode4(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
+                                               q8_encode4(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse));
+  else
+    *reinterpret_cast<uint16_t*>(to) = (uint16_t)q8_encode2(x[0] * inverse, x[1] * inverse);
+}
+
+// Whole heads rotated, d a power of two from 16 to 256 (128 for parts: a row's lanes are one warp's), everything on the boundaries of its vectors: d / (2 N) lanes a row, each
+// with N elements of its first half and the N that they turn with.  N = 8 (16 bytes of bfloat16 a load) for rows; N = 2 for
+// parts, whose steps have few rows: four times the lanes then share the sums.
+template <typename T, bool PARTS, int N>
+__global__ void __launch_bounds__(PARTS ? FEW_THREADS : THREADS) store_vec_kernel(const Store s) {
+  pdl_trigger();
+  pdl_wait();
+  const int lanes = s.d / (2 * N), half = s.d / 2, heads = s.n_q + 2 * s.n_kv;
+  const long long unit = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long row = unit / lanes;
+  if ((unit & ~31LL) / lanes >= (long long)s.tokens * heads) return;      // the whole warp
+  const bool there = row < (long long)s.tokens * heads;
+  const int token = there ? (int)(row / heads) : s.tokens - 1, head = there ? (int)(row - (long long)token * heads) : heads - 1;
+  const int at = (int)(unit % lanes) * N;
+  float lo[N], hi[N];
+  take<T, PARTS, N>(s, token, head * s.d + at, lo);
+  take<T, PARTS, N>(s, token, head * s.d + at + half, hi);
+  float2 turn[N];
+  if (head < s.n_q + s.n_kv) {
+    const float4* t = reinterpret_cast<const float4*>(s.table + (size_t)token * half + at);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      const float4 f = t[j];
+      turn[2 * j] = make_float2(f.x, f.y), turn[2 * j + 1] = make_float2(f.z, f.w);
+    }
+  }
+  const bool stored = head >= s.n_q;
+  if (head < s.n_q) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) rope_rotate(lo[j], hi[j], turn[j].x, turn[j].y, lo[j], hi[j]);
+    using O = T;
+    O* to = static_cast<O*>(s.q_out) + (size_t)token * s.n_q * s.d + head * s.d + at;
+    if (there) put<N>(to, lo), put<N>(to + half, hi);
+  } else if (head < s.n_q + s.n_kv) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const double a = lo[j], b = hi[j], c = turn[j].x, n = turn[j].y;
+      lo[j] = q8_to_odd(a * c - b * n);
+      hi[j] = q8_to_odd(b * c + a * n);
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = max(top, max(__float_as_uint(lo[j]) & 0x7fffffffu, __float_as_uint(hi[j]) & 0x7fffffffu));
+  for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (!there || !stored) return;
+  const bool is_v = head >= s.n_q + s.n_kv;
+  const long long place = pool_row(s, token, head - s.n_q - (is_v ? s.n_kv : 0), at == 0);
+  if (place < 0) return;
+  const int byte = q8_byte(top);
+  if (byte == Q8_NAN_BYTE) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) lo[j] = hi[j] = 0.f;
+  }
+  const float inverse = byte == Q8_NAN_BYTE ? 0.f : q8_inverse(byte);
+  uint8_t* to = (is_v ? s.v : s.k) + place * s.d + at;
+  put_codes<N>(to, lo, inverse);
+  put_codes<N>(to + half, hi, inverse);
+  if (at == 0) (is_v ? s.v_scale : s.k_scale)[place] = (uint8_t)byte;
+}
+
+// Any head size up to 256, any rotary_dim, any alignment: a warp a row, a lane every 32nd element.
+template <typename T, bool PARTS>
+__global__ void __launch_bounds__(THREADS) store_any_kernel(const Store s) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int EACH = MOST_DIM / 32;
+  const int heads = s.n_q + 2 * s.n_kv, lane = threadIdx.x & 31, half = s.rotary_dim / 2;
+  const long long row = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  if (row >= (long long)s.tokens * heads) return;
+  const int token = (int)(row / heads), head = (int)(row - (long long)token * heads);
+  const bool turns = head < s.n_q + s.n_kv, is_q = head < s.n_q;
+  float x[EACH];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int i = j * 32 + lane;
+    x[j] = 0.f;
+    if (i >= s.d) continue;
+    float own[1];
+    take<T, PARTS, 1>(s, token, head * s.d + i, own);
+    x[j] = own[0];
+    if (turns && i < 2 * half) {
+      const int pair = i < half ? i : i - half;
+      float other[1];
+      take<T, PARTS, 1>(s, token, head * s.d + (i < half ? i + half : i - half), other);
+      const float2 f = s.table[(size_t)token * half + pair];
+      if (is_q) {
+        float rlo, rhi;
+        rope_rotate(i < half ? own[0] : other[0], i < half ? other[0] : own[0], f.x, f.y, rlo, rhi);
+        x[j] = i < half ? rlo : rhi;
+      } else {
+        const double a = own[0], b = other[0], c = f.x, n = f.y;
+        x[j] = q8_to_odd(i < half ? a * c - b * n : a * c + b * n);
+      }
+    }
+    top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+  }
+  if (is_q) {
+    T* to = static_cast<T*>(s.q_out) + (size_t)token * s.n_q * s.d + head * s.d;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+      if (j * 32 + lane < s.d) to[j * 32 + lane] = from_f32<T>(x[j]);
+    return;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool is_v = !turns;
+  const long long place = pool_row(s, token, head - s.n_q - (is_v ? s.n_kv : 0), lane == 0);
+  if (place < 0) return;
+  const int byte = q8_byte(top);
+  const float inverse = byte == Q8_NAN_BYTE ? 0.f : q8_inverse(byte);
+  uint8_t* to = (is_v ? s.v : s.k) + place * s.d;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j)
+    if (j * 32 + lane < s.d) to[j * 32 + lane] = (uint8_t)q8_encode2(byte == Q8_NAN_BYTE ? 0.f : x[j] * inverse, 0.f);
+  if (lane == 0) (is_v ? s.v_scale : s.k_scale)[place] = (uint8_t)byte;
+}
+
+template <typename T, bool PARTS>
+int launch_store(const Store& s, bool vec, cudaStream_t stream) {
+  const long long rows = (long long)s.tokens * (s.n_q + 2 * s.n_kv);
+  constexpr int N = PARTS ? 2 : 8, threads = PARTS ? FEW_THREADS : THREADS;
+  if (vec) {
+    const long long units = rows * (s.d / (2 * N));
+    return (int)lab_launch(store_vec_kernel<T, PARTS, N>, dim3((unsigned)((units + threads - 1) / threads)), dim3(threads), 0, stream, s);
+  }
+  return (int)lab_launch(store_any_kernel<T, PARTS>, dim3((unsigned)((rows + THREADS / 32 - 1) / (THREADS / 32))), dim3(THREADS), 0, stream, s);
+}
+
+// ----------------------------------------------------------------------------------------
+// Reading back: a thread takes N codes of a key and leaves 16 bytes (N = 1: any size and alignment).
+// ----------------------------------------------------------------------------------------
+template <typename T, int N>
+__global__ void __launch_bounds__(THREADS) load_kernel(T* __restrict__ out_k, T* __restrict__ out_v, const uint8_t* __restrict__ k,
+                                                       const uint8_t* __restrict__ v, const uint8_t* __restrict__ k_scale,
+                                                       const uint8_t* __restrict__ v_scale, const int* __restrict__ slots, long long rows,
+                                                       int n_kv, int d, int page_size, int num_pages) {
+  pdl_trigger();
+  pdl_wait();
+  const int pieces = d / N;
+  const long long unit = (long long)blockIdx.x * THREADS + threadIdx.x;
+  const long long head_row = unit / pieces;
+  if (head_row >= rows * n_kv) return;
+  const int at = (int)(unit - head_row * pieces) * N;
+  const long long row = head_row / n_kv;
+  const int head = (int)(head_row - row * n_kv), slot = slots[row];
+  const int page = slot >= 0 ? slot / page_size : -1;
+  if (page >= num_pages && at == 0) lab_set_error(LAB_ERR_PAGE_RANGE);
+  const bool held = page >= 0 && page < num_pages;
+  const long long place = held ? ((long long)page * n_kv + head) * page_size + (slot - page * page_size) : 0;
+  auto one = [&](T* out, const uint8_t* codes, const uint8_t* scales) {
+    const float f = held ? q8_scale(scales[place]) : 0.f;
+    T* to = out + head_row * d + at;
+    const uint8_t* from = codes + place * d + at;
+    if constexpr (N == 8) {
+      const uint2 c = held ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+      const float4 a = q8_decode4(c.x), b = q8_decode4(c.y);
+      const float x[8] = {a.x * f, a.y * f, a.z * f, a.w * f, b.x * f, b.y * f, b.z * f, b.w * f};
+      put<8>(to, x);
+    } else if constexpr (N == 4) {
+      const uint32_t c = held ? *reinterpret_cast<const uint32_t*>(from) : 0u;
+      const float4 a = q8_decode4(c);
+      store4(to, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
+    } else {
+      to[0] = from_f32<T>(held ? q8_decode(from[0]) * f : 0.f);
+    }
+  };
+  one(out_k, k, k_scale);
+  one(out_v, v, v_scale);
+}
+
+template <typename T>
+int launch_load(T* out_k, T* out_v, const uint8_t* k, const uint8_t* v, const uint8_t* k_scale, const uint8_t* v_scale, const int* slots,
+                long long rows, int n_kv, int d, int page_size, int num_pages, cudaStream_t stream) {
+  constexpr int N = 16 / sizeof(T);
+  const bool vec = d % N == 0 && ((((uintptr_t)out_k) | ((uintptr_t)out_v)) & 15) == 0 && ((((uintptr_t)k) | ((uintptr_t)v)) & (N - 1)) == 0;
+  const long long units = rows * n_kv * (vec ? d / N : d);
+  const dim3 grid((unsigned)((units + THREADS - 1) / THREADS));
+  return (int)lab_launch(vec ? load_kernel<T, N> : load_kernel<T, 1>, grid, dim3(THREADS), 0, stream, out_k, out_v, k, v, k_scale, v_scale,
+                         slots, rows, n_kv, d, page_size, num_pages);
+}
+
+}  // namespace
+
+LAB_EXPORT int lab_q8_most_dim() { return MOST_DIM; }
+
+// rows: [tokens, row_stride] of `dtype`, or (parts > 0) [parts, tokens, width] floats whose sum with `bias` is rounded to
+// bfloat16 first; width = (n_q + 2 n_kv) d.  table: [tokens, rotary_dim / 2] (cos, sin).  q_out: [tokens, n_q * d].  Slots that
+// are not negative differ from one another.
+LAB_EXPORT int lab_rope_kv_store_q8(const void* rows, long long row_stride, int parts, long long part_stride, const void* bias,
+                                    const void* table, int rotary_dim, const int* slots, void* q_out, void* k, void* v, void* k_scale,
+                                    void* v_scale, int tokens, int n_q, int n_kv, int d, int page_size, int num_pages, int dtype,
+                                    cudaStream_t stream) {
+  if (tokens <= 0) return 0;
+  if (d < 1 || d > MOST_DIM || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > d || n_q < 0 || n_kv < 1 || page_size < 1 || num_pages < 0 ||
+      parts < 0 || (parts > 0 && dtype != LAB_BF16) || (rotary_dim > 0 && table == nullptr))
+    return (int)cudaErrorInvalidValue;
+  Store s;
+  s.rows = rows, s.row_stride = row_stride, s.parts = parts, s.part_stride = part_stride, s.bias = (const __nv_bfloat16*)bias;
+  s.table = (const float2*)table, s.rotary_dim = rotary_dim, s.slots = slots, s.q_out = q_out;
+  s.k = (uint8_t*)k, s.v = (uint8_t*)v, s.k_scale = (uint8_t*)k_scale, s.v_scale = (uint8_t*)v_scale;
+  s.tokens = tokens, s.n_q = n_q, s.n_kv = n_kv, s.d = d, s.page_size = page_size, s.num_pages = num_pages;
+  const int size = parts > 0 || dtype == LAB_F32 ? 4 : 2;
+  const bool vec = rotary_dim == d && d >= 16 && d <= (parts > 0 ? 128 : 256) && (d & (d - 1)) == 0 && row_stride * size % 16 == 0 &&
+                   (parts == 0 || part_stride * size % 16 == 0) &&
+                   (((uintptr_t)rows | (uintptr_t)table | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
+  if (dtype == LAB_F32) return launch_store<float, false>(s, vec, stream);
+  return parts > 0 ? launch_store<__nv_bfloat16, true>(s, vec, stream) : launch_store<__nv_bfloat16, false>(s, vec, stream);
+}
+
+// out_k, out_v: [rows, n_kv, d] of `dtype`; a negative slot gives a row of zeros.
+LAB_EXPORT int lab_kv_load_q8(void* out_k, void* out_v, const void* k, const void* v, const void* k_scale, const void* v_scale,
+                              const int* slots, long long rows, int n_kv, int d, int page_size, int num_pages, int dtype,
+                              cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (d < 1 || n_kv < 1 || page_size < 1 || num_pages < 0) return (int)cudaErrorInvalidValue;
+  const uint8_t *kc = (const uint8_t*)k, *vc = (const uint8_t*)v, *ks = (const uint8_t*)k_scale, *vs = (const uint8_t*)v_scale;
+  if (dtype == LAB_F32)
+    return launch_load((float*)out_k, (float*)out_v, kc, vc, ks, vs, slots, rows, n_kv, d, page_size, num_pages, stream);
+  return launch_load((__nv_bfloat16*)out_k, (__nv_bfloat16*)out_v, kc, vc, ks, vs, slots, rows, n_kv, d, page_size, num_pages, stream);
+}

@@ -1,0 +1,311 @@
+// Drafted tokens against the target's probabilities.
+//
+// A request brings its rows of logits, one after the token it holds and one after each drafted token; draft x_i is judged by row
+// i.  With p = softmax(logits / T) and q the probabilities that the draft was drawn from (or all of it on x_i):
+//   accept x_i while u_i q(x_i) < p(x_i); at the first refusal, and after the last row, draw the token that ends the request:
+//   argmax_t w_t / E_t with w = max(p - q, 0) at a refusal and w = p after the last row, E_t = -log(u_t) exponential.
+// What comes out is distributed as the target's own draws are.  Where w is nothing anywhere (p = q up to rounding) w = p.
+// T = 0: accept while x_i is the argmax of its row, and end with the argmax (ties: the smallest index; a NaN never wins, and a
+// row without any number gives INT32_MAX, as the sampling kernel does).
+// The u come from the sampling kernel's hash of (seed, position, t), so a draw depends on neither the batch nor the step; u_i of
+// the test is the hash of the row's key's complement.  Probabilities are 32-bit: a test or a draw goes another way than in
+// exact arithmetic only where two numbers agree to about 2^-20.
+//
+// Two launches: the rows' largest entry and sum of exponentials by chunk (every logit read once: the bound, memory), then a
+// cluster of eight CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that is
+// left (its logits come from L2).  Partial results lie in the caller's scratch and nothing has to be zero before a call, so calls
+// on several streams, or from several graphs, do not meet.
+#include <limits.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int CHUNK = 8192, STAT_THREADS = 256, PICK_THREADS = 512, CLUSTER = 8;
+constexpr int ROUNDS = CHUNK / (STAT_THREADS * 4);
+
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x7FEB352Du;
+  x ^= x >> 15;
+  x *= 0x846CA68Bu;
+  x ^= x >> 16;
+  return x;
+}
+__device__ __forceinline__ float uniform_of(uint32_t h) { return ((float)(h >> 9) + 0.5f) * (1.f / 8388608.f); }
+__device__ __forceinline__ bool better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
+
+struct Args {
+  const float* logits;
+  long long ld;
+  const float* draft_probs;   // null: the drafts are certain
+  long long ld_probs;
+  const int *drafts, *starts;
+  const float* temperature;   // [requests], null: all 0
+  const uint32_t* seeds;
+  const int* positions;       // of the token that a request's first row decides
+  int rows, vocab, requests, chunks;
+  float4* part;               // [rows, chunks]: largest entry, sum of exponentials relative to it, its index
+  int *tokens, *counts;
+};
+
+// A request's rows, none where `starts` is not ascending within the logits.
+__device__ __forceinline__ int2 rows_of(const Args& a, int b) {
+  const int lo = a.starts[b], hi = a.starts[b + 1];
+  return lo < 0 || hi > a.rows || hi < lo ? make_int2(0, 0) : make_int2(lo, hi);
+}
+
+__global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args a) {
+  __shared__ float sm[STAT_THREADS / 32], ss[STAT_THREADS / 32];
+  __shared__ int si[STAT_THREADS / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float inverse = 0.f;
+  if (a.temperature != nullptr) {
+    int b = 0, past = a.requests;
+    while (past - b > 1) {
+      const int mid = (b + past) / 2;
+      if (a.starts[mid] <= row) b = mid; else past = mid;
+    }
+    const float t = a.temperature[b];
+    inverse = t > 0.f ? 1.f / t : 0.f;
+  }
+  const bool greedy = inverse == 0.f;
+  const float* lr = a.logits + (size_t)row * a.ld;
+  const int first = chunk * CHUNK, end = min(a.vocab, first + CHUNK);
+  float x[4 * ROUNDS];
+  const bool vec = (a.ld & 3) == 0 && (((uintptr_t)a.logits) & 15) == 0;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = first + (r * STAT_THREADS + (int)threadIdx.x) * 4;
+    if (vec && i + 3 < end) {
+      const float4 v = load4(lr + i);
+      x[4 * r] = v.x, x[4 * r + 1] = v.y, x[4 * r + 2] = v.z, x[4 * r + 3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * r + e] = i + e < end ? lr[i + e] : __uint_as_float(0x7fffffffu);
+    }
+  }
+  float m = -INFINITY;
+  int at = INT_MAX;
+  if (greedy) {
+#pragma unroll
+    for (int j = 0; j < 4 * ROUNDS; ++j) {
+      const int i = first + ((j >> 2) * STAT_THREADS + (int)threadIdx.x) * 4 + (j & 3);
+      if (better(x[j], i, m, at)) m = x[j], at = i;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4 * ROUNDS; ++j) {
+      x[j] *= inverse;
+      m = fmaxf(m, x[j]);      // (a NaN is passed over)
+    }
+  }
+  float sum = 0.f;
+  if (!greedy) {
+#pragma unroll
+    for (int j = 0; j < 4 * ROUNDS; ++j) sum += x[j] == m ? 1.f : x[j] == x[j] ? __expf(x[j] - m) : 0.f;
+  }
+  auto join = [&](float om, float os, int oi) {
+    if (greedy) {
+      if (better(om, oi, m, at)) m = om, at = oi;
+      return;
+    }
+    const float big = fmaxf(m, om);
+    sum = (m == big ? sum : sum * __expf(m - big)) + (om == big ? os : os * __expf(om - big));
+    m = big;
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), __shfl_xor_sync(0xffffffffu, at, o));
+  if (lane == 0) sm[warp] = m, ss[warp] = sum, si[warp] = at;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < STAT_THREADS / 32; ++w) join(sm[w], ss[w], si[w]);
+  a.part[(size_t)row * a.chunks + chunk] = make_float4(m, sum, __int_as_float(at), 0.f);
+}
+
+// A row's largest entry, its index, and its sum of exponentials, by one warp in the order of the chunks' lanes.
+__device__ __forceinline__ float4 row_stats(const Args& a, int row, int lane) {
+  float m = -INFINITY, sum = 0.f;
+  int at = INT_MAX;
+  for (int c = lane; c < a.chunks; c += 32) {
+    const float4 p = a.part[(size_t)row * a.chunks + c];
+    const int i = __float_as_int(p.z);
+    const float big = fmaxf(m, p.x);
+    sum = (m == big ? sum : sum * expf(m - big)) + (p.x == big ? p.y : p.y * expf(p.x - big));
+    if (better(p.x, i, m, at)) at = i;
+    m = big;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, at, o);
+    const float big = fmaxf(m, om);
+    if (better(om, oi, m, at)) at = oi;
+    sum = (m == big ? sum : sum * expf(m - big)) + (om == big ? os : os * expf(om - big));
+    m = big;
+  }
+  return make_float4(m, sum, __int_as_float(at), 0.f);
+}
+
+struct Best {
+  float v, pv;      // of the weights left, and of p
+  int i, pi;
+  __device__ __forceinline__ void join(const Best& o) {
+    if (better(o.v, o.i, v, i)) v = o.v, i = o.i;
+    if (better(o.pv, o.pi, pv, pi)) pv = o.pv, pi = o.pi;
+  }
+};
+
+__global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a, int cluster) {
+  __shared__ int stop_s, greedy_s;
+  __shared__ float m_s, inverse_sum_s;
+  __shared__ Best warp_s[PICK_THREADS / 32];
+  __shared__ Best cta_s[CLUSTER];
+  pdl_trigger();
+  if (cluster > 1) cluster_sync();      // every CTA is there before another writes to it
+  pdl_wait();
+  const int b = blockIdx.x / cluster, part = blockIdx.x - b * cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int2 span = rows_of(a, b);
+  const int n = span.y - span.x;
+  const float t = a.temperature != nullptr ? a.temperature[b] : 0.f, inverse = t > 0.f ? 1.f / t : 0.f;
+  const bool greedy = inverse == 0.f;
+  if (threadIdx.x == 0) {
+    stop_s = max(n - 1, 0);
+    if (part == 0 && (a.starts[b] < 0 || a.starts[b + 1] > a.rows || a.starts[b + 1] < a.starts[b])) lab_set_error(LAB_ERR_ROW_RANGE);
+  }
+  __syncthreads();
+  auto key_of = [&](int i) { return mix32(mix32(a.seeds[b] ^ 0x9E3779B9u) ^ (uint32_t)(a.positions[b] + i)); };
+  for (int i = warp; i < n - 1; i += PICK_THREADS / 32) {
+    const int row = span.x + i, x = a.drafts[row];
+    const float4 s = row_stats(a, row, lane);
+    bool taken = x >= 0 && x < a.vocab;
+    if (greedy) {
+      taken = taken && x == __float_as_int(s.z);
+    } else if (taken) {
+      const float v = a.logits[(size_t)row * a.ld + x] * inverse;
+      const float p = (v == s.x ? 1.f : expf(v - s.x)) / s.y;
+      const float q = a.draft_probs != nullptr ? a.draft_probs[(size_t)row * a.ld_probs + x] : 1.f;
+      taken = uniform_of(mix32(~key_of(i))) * q < p;
+    }
+    if (!taken && lane == 0) atomicMin(&stop_s, i);
+  }
+  __syncthreads();
+  const int stop = stop_s, row = span.x + stop;
+  if (warp == 0 && n > 0) {
+    const float4 s = row_stats(a, row, lane);
+    if (lane == 0) m_s = s.x, inverse_sum_s = 1.f / s.y, greedy_s = __float_as_int(s.z);
+  }
+  __syncthreads();
+  Best best = {0.f, 0.f, INT_MAX, INT_MAX};      // a weight above 0 is wanted
+  if (!greedy && n > 0) {
+    const float m = m_s, inverse_sum = inverse_sum_s;
+    const uint32_t key = key_of(stop);
+    const float* lr = a.logits + (size_t)row * a.ld;
+    const bool over = stop == n - 1;
+    const float* qr = !over && a.draft_probs != nullptr ? a.draft_probs + (size_t)row * a.ld_probs : nullptr;
+    const int certain = !over && a.draft_probs == nullptr ? a.drafts[row] : -1;
+    auto consider = [&](float logit, float q, int i) {
+      const float v = logit * inverse;
+      const float p = (v == m ? 1.f : expf(v - m)) * inverse_sum;
+      const float w = i == certain ? 0.f : fmaxf(p - q, 0.f);
+      const float rate = __fdividef(1.f, -logf(uniform_of(mix32(key + (uint32_t)i * 0x85EBCA6Bu))));
+      if (better(w * rate, i, best.v, best.i)) best.v = w * rate, best.i = i;
+      if (better(p * rate, i, best.pv, best.pi)) best.pv = p * rate, best.pi = i;
+    };
+    const bool vec = (a.ld & 3) == 0 && (((uintptr_t)a.logits) & 15) == 0 &&
+                     (qr == nullptr || ((a.ld_probs & 3) == 0 && (((uintptr_t)a.draft_probs) & 15) == 0));
+    for (int i = (part * PICK_THREADS + (int)threadIdx.x) * 4; i < a.vocab; i += cluster * PICK_THREADS * 4) {
+      if (vec && i + 3 < a.vocab) {
+        const float4 v = load4(lr + i), q = qr != nullptr ? load4(qr + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        consider(v.x, q.x, i);
+        consider(v.y, q.y, i + 1);
+        consider(v.z, q.z, i + 2);
+        consider(v.w, q.w, i + 3);
+      } else {
+        for (int e = i; e < min(i + 4, a.vocab); ++e) consider(lr[e], qr != nullptr ? qr[e] : 0.f, e);
+      }
+    }
+  }
+  auto over_lanes = [&]() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      Best other;
+      other.v = __shfl_xor_sync(0xffffffffu, best.v, o), other.i = __shfl_xor_sync(0xffffffffu, best.i, o);
+      other.pv = __shfl_xor_sync(0xffffffffu, best.pv, o), other.pi = __shfl_xor_sync(0xffffffffu, best.pi, o);
+      best.join(other);
+    }
+  };
+  over_lanes();
+  if (lane == 0) warp_s[warp] = best;
+  __syncthreads();
+  if (warp == 0) {
+    best = lane < PICK_THREADS / 32 ? warp_s[lane] : Best{0.f, 0.f, INT_MAX, INT_MAX};
+    over_lanes();
+    if (cluster > 1 && lane == 0) {
+      const uint32_t to = map_to_rank(smem_u32(&cta_s[part]), 0);
+      st_cluster_f32(to, best.v);
+      st_cluster_f32(to + 4, best.pv);
+      st_cluster_f32(to + 8, __int_as_float(best.i));
+      st_cluster_f32(to + 12, __int_as_float(best.pi));
+    }
+  }
+  if (cluster > 1) {
+    cluster_sync();
+    if (part != 0) return;
+    if (warp == 0)
+      for (int c = 0; c < cluster; ++c) best.join(cta_s[c]);
+  }
+  if (n == 0) {
+    if (threadIdx.x == 0) a.counts[b] = 0;
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += PICK_THREADS)
+    if (i != stop) a.tokens[span.x + i] = i < stop ? a.drafts[span.x + i] : -1;
+  if (threadIdx.x == 0) {
+    a.tokens[row] = greedy ? greedy_s : best.v > 0.f ? best.i : best.pi;
+    a.counts[b] = stop + 1;
+  }
+}
+
+}  // namespace
+
+// Bytes of scratch a call needs.
+LAB_EXPORT long long lab_verify_scratch(int rows, int vocab) { return (long long)rows * ((vocab + CHUNK - 1) / CHUNK) * 16; }
+
+// logits [rows, vocab] 32-bit, rows `ld` apart; draft_probs likewise or null; drafts [rows]: the token drafted after a row's (a
+// request's last row has none); starts [requests + 1]; temperature, seeds, positions [requests], null: greedy.  tokens [rows]:
+// what a request's rows give, drafts that were accepted, the token that ends it, -1 behind it; counts [requests].
+LAB_EXPORT int lab_verify_drafts(int* tokens, int* counts, const float* logits, long long ld, const float* draft_probs, long long ld_probs,
+                                 const int* drafts, const int* starts, const float* temperature, const uint32_t* seeds,
+                                 const int* positions, int rows, int vocab, int requests, void* scratch, cudaStream_t stream) {
+  if (requests <= 0) return 0;
+  if (rows < 0 || rows > 65535 || vocab < 1 || (rows > 0 && scratch == nullptr) || (((uintptr_t)scratch) & 15) ||
+      (temperature != nullptr && (seeds == nullptr || positions == nullptr)))
+    return (int)cudaErrorInvalidValue;
+  Args a;
+  a.logits = logits, a.ld = ld, a.draft_probs = draft_probs, a.ld_probs = ld_probs, a.drafts = drafts, a.starts = starts;
+  a.temperature = temperature, a.seeds = seeds, a.positions = positions;
+  a.rows = rows, a.vocab = vocab, a.requests = requests, a.chunks = (vocab + CHUNK - 1) / CHUNK;
+  a.part = (float4*)scratch, a.tokens = tokens, a.counts = counts;
+  if (rows > 0) {
+    const cudaError_t e = lab_launch(verify_chunks_kernel, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
+    if (e != cudaSuccess) return (int)e;
+  }
+  const int cluster = temperature != nullptr ? CLUSTER : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(requests * cluster);
+  cfg.blockDim = dim3(PICK_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_lab_pdl ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, verify_pick_kernel, a, cluster);
+}

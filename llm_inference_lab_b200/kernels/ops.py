@@ -11,6 +11,7 @@ import ctypes
 import functools
 import math
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -2330,3 +2331,212 @@ def memory_finish(o: torch.Tensor, m: torch.Tensor, gate: torch.Tensor, weight: 
         ctypes.c_float(q_scale), ctypes.c_float(floor), ctypes.c_float(eps), ctypes.c_float(mult),
         _ptr(ctx.row_req), _ptr(ctx.state_slot), dtype_code(weight.dtype), _stream()), "memory_finish")
     return out
+
+
+# ----------------------------------------------------------------------------------------
+# A cache in 8 bits (csrc/kernels/quant8.cuh): keys and values as codes of 1 sign, 4 exponent and 3 mantissa bits with one
+# scale byte e a row (a token's key or value of one kv head), a number being code * 2^(e - 127).  Half the memory and half the
+# bytes of a step of bfloat16 pages; what is read back is a bfloat16 exactly.
+# ----------------------------------------------------------------------------------------
+class QuantPages(NamedTuple):
+    """Pages of keys and values in 8 bits: codes [pages, n_kv, page_size, head_dim], scale bytes [pages, n_kv, page_size]."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def quant_pages(num_pages: int, n_kv: int, page_size: int, head_dim: int, device) -> QuantPages:
+    """New pages, with nothing in them: what may be read is decided by lengths and slots alone."""
+    shape = (int(num_pages), int(n_kv), int(page_size), int(head_dim))
+    code = lambda: torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)  # noqa: E731
+    byte = lambda: torch.empty(shape[:3], dtype=torch.uint8, device=device)  # noqa: E731
+    return QuantPages(code(), code(), byte(), byte())
+
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def _same_device(what: str, first: torch.Tensor, *tensors) -> None:
+    """All on the device of `first`, which is the current one: the kernel is launched on the current stream."""
+    _on_gpu(first, *tensors)
+    _require(all(t is None or t.device == first.device for t in tensors), f"{what}: tensors on different devices")
+    _require(first.device.index == torch.cuda.current_device(),
+             f"{what}: tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _q8_pages(what: str, pages: QuantPages, n_kv: int, head_dim: int) -> tuple[int, int]:
+    """Checks a cache's pages; (pages, page size)."""
+    _require(pages.k.dim() == 4 and tuple(pages.k.shape[1::2]) == (n_kv, head_dim),
+             f"{what}: pages of shape {tuple(pages.k.shape)} are not [pages, {n_kv}, page_size, {head_dim}]")
+    for t, dtype, shape in ((pages.k, torch.float8_e4m3fn, pages.k.shape), (pages.v, torch.float8_e4m3fn, pages.k.shape),
+                            (pages.k_scale, torch.uint8, pages.k.shape[:3]), (pages.v_scale, torch.uint8, pages.k.shape[:3])):
+        _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
+                 f"{what}: pages hold contiguous float8_e4m3fn codes and uint8 scales of one shape, got {t.dtype} {tuple(t.shape)}")
+    return pages.k.shape[0], pages.k.shape[2]
+
+
+def _integers(what: str, name: str, t: torch.Tensor, count: int) -> None:
+    _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= count,
+             f"{what}: {name} holds {count} int32 numbers or more, contiguous, got {t.dtype} {tuple(t.shape)}")
+
+
+def rope_kv_store_q8(qkv: torch.Tensor, table: torch.Tensor | None, rotary_dim: int, slots: torch.Tensor, pages: QuantPages, n_q: int,
+                     n_kv: int, head_dim: int, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotates q and k, writes k and v in 8 bits to their cache slots (a negative slot: nowhere), and returns the rotated q
+    [tokens, n_q * head_dim]; `qkv` stays as it is.
+
+    `qkv` is the fused projection [tokens, (n_q + 2 n_kv) * d], bfloat16 or float32, or its 32-bit partial products [parts,
+    tokens, ..] whose sum with `bias` is rounded to bfloat16 first (contiguous); `table` comes from `rope_table` (None with
+    rotary_dim 0).  Slots that are not negative differ from one another.  A code is what the exact rotated number rounds to, in
+    one rounding; a row with a number that is not finite reads back as NaN.  Head sizes up to 256."""
+    what = "rope_kv_store_q8"
+    parts = qkv.shape[0] if qkv.dim() == 3 else 0
+    _require(qkv.dim() in (2, 3), f"{what}: rows or partial products, got {tuple(qkv.shape)}")
+    tokens, width = qkv.shape[-2], (n_q + 2 * n_kv) * head_dim
+    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
+    _require( qkv.shape[-1] == width and qkv.stride(-1) == 1,
+             f"{what}: rows of {width} = (n_q + 2 n_kv) * head_dim neighbouring numbers, got {tuple(qkv.shape)}")
+    _require(parts == 0 or (qkv.dtype == torch.float32 and qkv.is_contiguous()), f"{what}: partial products are contiguous float32")
+    _require(bias is None or (parts > 0 and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == width),
+             f"{what}: a bias of {width} bfloat16 numbers goes with partial products")
+    _require(0 <= rotary_dim <= head_dim <= 256 and rotary_dim % 2 == 0, f"{what}: head size {head_dim} up to 256, rotary_dim {rotary_dim} even")
+    _require(rotary_dim == 0 or (table is not None and table.dtype == torch.float32 and table.is_contiguous()
+                                 and tuple(table.shape) == (tokens, rotary_dim // 2, 2)),
+             f"{what}: a table [{tokens}, {rotary_dim // 2}, 2] of cosines and sines, float32 and contiguous")
+    _integers(what, "slots", slots, tokens)
+    dt = torch.bfloat16 if parts else qkv.dtype
+    code = dtype_code(dt)
+    _same_device(what, qkv, table, slots, bias, *pages)
+    q = torch.empty((tokens, n_q * head_dim), dtype=dt, device=qkv.device)
+    _check(lib("quant_cache").lab_rope_kv_store_q8(
+        _ptr(qkv), ctypes.c_longlong(qkv.stride(-2)), parts, ctypes.c_longlong(tokens * width), _ptr(bias), _ptr(table if rotary_dim else None),
+        rotary_dim, _ptr(slots), _ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), tokens, n_q, n_kv,
+        head_dim, page_size, num_pages, code, _stream()), what)
+    return q
+
+
+def kv_load_q8(pages: QuantPages, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values at `slots` of an 8-bit cache as numbers: k, v [rows, n_kv, head_dim] of `dtype` (both types hold them
+    exactly).  A negative slot gives a row of zeros; a slot may come more than once."""
+    what = "kv_load_q8"
+    _require(pages.k.dim() == 4, f"{what}: pages of shape {tuple(pages.k.shape)} are not [pages, n_kv, page_size, head_dim]")
+    n_kv, head_dim = pages.k.shape[1], pages.k.shape[3]
+    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
+    _require(slots.dim() == 1, f"{what}: one row of slots")
+    _integers(what, "slots", slots, slots.numel())
+    rows, code = slots.numel(), dtype_code(dtype)
+    _same_device(what, slots, *pages)
+    k = torch.empty((rows, n_kv, head_dim), dtype=dtype, device=slots.device)
+    v = torch.empty_like(k)
+    _check(lib("quant_cache").lab_kv_load_q8(
+        _ptr(k), _ptr(v), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(slots), ctypes.c_longlong(rows),
+        n_kv, head_dim, page_size, num_pages, code, _stream()), what)
+    return k, v
+
+
+def q8_few_width(rows: int) -> int:
+    """Rows (tokens times query heads of a kv head) that a CTA of the few-rows kernel takes, for requests of `rows` at most."""
+    return 16 if rows <= 16 else 32 if rows <= 32 else 48
+
+
+def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
+    """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once."""
+    room = (2 if width <= 32 else 1) * sm_count()
+    return max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
+
+
+def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_len: torch.Tensor, pos0: torch.Tensor,
+                 block_table: torch.Tensor, n_requests: int, q_lens, max_kv_len: int, n_q: int, n_kv: int, head_dim: int, window: int,
+                 scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of every row over its request's keys in an 8-bit cache: all of them, the last `window`, or (a negative
+    `window`) those of the row's own chunk of that many positions.  Arguments as `attention_tc`: request b's rows of q are
+    q_start[b] .. q_start[b + 1], at positions pos0[b] on; keys from kv_len[b] on do not exist; `q_lens` are the host's row
+    counts.  A row that sees no key is 0; rows of no request stay as they are.
+
+    bfloat16 queries of heads of 64 and 128 over pages of 8 to 128 (a power of two) run on the tensor cores; 32-bit queries (in
+    32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units."""
+    what = "attention_q8"
+    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
+    tokens, width = q.shape[0], n_q * head_dim
+    _require(q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1, f"{what}: q of {width} neighbouring numbers a row, got {tuple(q.shape)}")
+    _require(n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
+    _require(scale > 0, f"{what}: the scale is positive")
+    for name, t, count in (("q_start", q_start, n_requests + 1), ("kv_len", kv_len, n_requests), ("pos0", pos0, n_requests)):
+        _integers(what, name, t, count)
+    _integers(what, "block_table", block_table, 0)
+    _require(block_table.dim() == 2 and block_table.shape[0] >= n_requests, f"{what}: a row of the block table per request")
+    _require(len(q_lens) == n_requests, f"{what}: the host's row counts, one per request")
+    _require(out is None or (out.dtype == q.dtype and tuple(out.shape) == (tokens, width) and out.stride(1) == 1), f"{what}: out as q")
+    code = dtype_code(q.dtype)
+    _same_device(what, q, q_start, kv_len, pos0, block_table, out, *pages)
+    if out is None:
+        out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
+    if not q_lens or max(q_lens) == 0 or tokens == 0:
+        return out
+    if code == BF16 and not _force_plain and head_dim in (64, 128) and page_size in (8, 16, 32, 64, 128) and q.stride(0) % 2 == 0 \
+            and q.data_ptr() % 4 == 0 and block_table.shape[1] > 0 and num_pages > 0:
+        group, longest = n_q // n_kv, max(q_lens)
+        width = q8_few_width(longest * group)
+        ctas = sum(n_kv * -(-n * group // width) for n in q_lens)
+        splits = q8_few_splits(ctas, width, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest))
+        L = lib("attention_q8_few", {"LAB_HEAD_DIM": head_dim})
+        scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
+        _check(L.lab_attention_q8_few(
+            _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
+            _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q, n_kv,
+            page_size, num_pages, window, ctypes.c_float(scale), longest, longest, width, splits, _ptr(scratch), _stream()),
+            what, 2 if splits > 1 else 1)
+        return out
+    _check(lib("attention_q8").lab_attention_q8_any(
+        _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
+        _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q, n_kv,
+        head_dim, page_size, num_pages, window, ctypes.c_float(scale), code, _stream()), what)
+    return out
+
+
+# ----------------------------------------------------------------------------------------
+# Drafted tokens (csrc/kernels/verify.cu)
+# ----------------------------------------------------------------------------------------
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tensor, draft_probs: torch.Tensor | None = None,
+                  temperature: torch.Tensor | None = None, seeds: torch.Tensor | None = None, positions: torch.Tensor | None = None):
+    """Judges drafted tokens by the target's 32-bit logits [rows, vocab] and draws the token that follows the accepted ones.
+
+    Request b's rows are starts[b] .. starts[b + 1] (int32 [requests + 1], ascending): one after the token it holds, one after
+    each drafted token.  drafts [rows] int32: the token drafted after a row's; a request's last row has none, whatever stands
+    there.  `draft_probs` [rows, vocab] 32-bit: the probabilities each draft was drawn from (None: drafts are certain, as an
+    argmax or a copied n-gram is); `temperature`, `seeds`, `positions` per request as `sample` takes them, positions that of the
+    token a request's first row decides; no temperature, or 0: greedy.  Emitted tokens are distributed as the target's own.
+
+    Returns (tokens [rows], counts [requests]), int32: counts[b] tokens from row starts[b] on, drafts that were accepted and then
+    the drawn one, -1 behind them.  A row without any number gives INT32_MAX, as `sample` does."""
+    what = "verify_drafts"
+    _require(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1 and logits.shape[1] > 0,
+             f"{what}: logits are float32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    _integers(what, "drafts", drafts, rows)
+    _integers(what, "starts", starts, 1)
+    _require(rows <= 65535, f"{what}: up to 65535 rows, got {rows}")
+    requests = starts.numel() - 1
+    _require(draft_probs is None or (draft_probs.dtype == torch.float32 and draft_probs.shape == logits.shape and draft_probs.stride(1) == 1),
+             f"{what}: draft_probs are float32 of the logits' shape")
+    if temperature is not None:
+        _require(temperature.dtype == torch.float32 and temperature.is_contiguous() and temperature.numel() >= requests,
+                 f"{what}: a float32 temperature per request")
+        _require(seeds is not None and positions is not None, f"{what}: a temperature needs seeds and positions")
+        _integers(what, "seeds", seeds, requests)
+        _integers(what, "positions", positions, requests)
+    _same_device(what, logits, drafts, starts, draft_probs, temperature, seeds, positions)
+    tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    counts = torch.empty((requests,), dtype=torch.int32, device=logits.device)
+    L = lib("verify")
+    L.lab_verify_scratch.restype = ctypes.c_longlong
+    scratch = torch.empty((max(1, int(L.lab_verify_scratch(rows, vocab))),), dtype=torch.uint8, device=logits.device)
+    _check(L.lab_verify_drafts(
+        _ptr(tokens), _ptr(counts), _ptr(logits), ctypes.c_longlong(logits.stride(0)), _ptr(draft_probs),
+        ctypes.c_longlong(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(drafts), _ptr(starts), _ptr(temperature),
+        _ptr(seeds if temperature is not None else None), _ptr(positions if temperature is not None else None), rows, vocab, requests,
+        _ptr(scratch), _stream()), what, 2 if rows else 1)
+    return tokens, counts
