@@ -2437,6 +2437,10 @@ def kv_load_q8(pages: QuantPages, slots: torch.Tensor, dtype: torch.dtype = torc
     return k, v
 
 
+# Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, which splits the keys.
+Q8_FEW_ROWS = 128
+
+
 def q8_few_width(rows: int) -> int:
     """Rows (tokens times query heads of a kv head) that a CTA of the few-rows kernel takes, for requests of `rows` at most."""
     return 16 if rows <= 16 else 32 if rows <= 32 else 48
@@ -2478,17 +2482,25 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         return out
     if code == BF16 and not _force_plain and head_dim in (64, 128) and page_size in (8, 16, 32, 64, 128) and q.stride(0) % 2 == 0 \
             and q.data_ptr() % 4 == 0 and block_table.shape[1] > 0 and num_pages > 0:
-        group, longest = n_q // n_kv, max(q_lens)
-        width = q8_few_width(longest * group)
-        ctas = sum(n_kv * -(-n * group // width) for n in q_lens)
-        splits = q8_few_splits(ctas, width, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest))
-        L = lib("attention_q8_few", {"LAB_HEAD_DIM": head_dim})
-        scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
-        _check(L.lab_attention_q8_few(
-            _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
-            _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q, n_kv,
-            page_size, num_pages, window, ctypes.c_float(scale), longest, longest, width, splits, _ptr(scratch), _stream()),
-            what, 2 if splits > 1 else 1)
+        group = n_q // n_kv
+        # requests of up to `few` rows, and those of more
+        few = max(1, Q8_FEW_ROWS // group) if q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else max(q_lens)
+        longest, longest_few = max(q_lens), max((n for n in q_lens if n <= few), default=0)
+        if longest > few:
+            _check(lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim}).lab_attention_q8_rows(
+                _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
+                _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q,
+                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few + 1, longest, _stream()), what)
+        if longest_few:
+            width = q8_few_width(longest_few * group)
+            ctas = sum(n_kv * -(-n * group // width) for n in q_lens if n <= few)
+            splits = q8_few_splits(ctas, width, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few))
+            scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
+            _check(lib("attention_q8_few", {"LAB_HEAD_DIM": head_dim}).lab_attention_q8_few(
+                _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
+                _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q,
+                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few, longest_few, width, splits, _ptr(scratch), _stream()),
+                what, 2 if splits > 1 else 1)
         return out
     _check(lib("attention_q8").lab_attention_q8_any(
         _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
