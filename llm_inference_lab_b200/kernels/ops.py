@@ -2487,10 +2487,15 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         few = max(1, Q8_FEW_ROWS // group) if q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else max(q_lens)
         longest, longest_few = max(q_lens), max((n for n in q_lens if n <= few), default=0)
         if longest > few:
-            _check(lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim}).lab_attention_q8_rows(
+            L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
+            L.lab_attention_q8_rows_scratch.restype = ctypes.c_longlong
+            many = sum(1 for n in q_lens if n > few)
+            scratch = torch.empty((int(L.lab_attention_q8_rows_scratch(many, n_kv, window, max_kv_len, longest)),), dtype=torch.uint8, device=q.device)
+            _check(L.lab_attention_q8_rows(
                 _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
                 _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q,
-                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few + 1, longest, _stream()), what)
+                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few + 1, longest, many, max_kv_len, _ptr(scratch), _stream()),
+                what, 2)
         if longest_few:
             width = q8_few_width(longest_few * group)
             ctas = sum(n_kv * -(-n * group // width) for n in q_lens if n <= few)
