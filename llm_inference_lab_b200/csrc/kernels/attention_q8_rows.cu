@@ -6,16 +6,20 @@
 // and turning them anew in each CTA cost more than the attention's own arithmetic (measured, below).  The second is the
 // attention over those rows:
 //
-// A CTA takes 256 rows of one request and kv head, two groups of 128, and walks the keys in tiles of 128.  Row r is token r /
-// group and query head r % group of those that share the kv head, so a tile of keys is fetched once for all of them, and a
-// CTA's rows reach over few positions: only the last tiles of its walk (and a window's first) need a mask.
+// A CTA takes 128 rows of one request and kv head and walks the keys in tiles of 128.  Row r is token r / group and query head
+// r % group of those that share the kv head, so a tile of keys is fetched once for all of them, and a CTA's rows reach over few
+// positions: only the last tiles of its walk (and a window's first) need a mask.
 //   S = Q K^T       kind::f16, from shared memory
-//   P = softmax(S)  a thread a row: mask, running maximum and sum in 32 bits, 2^x, P rounded to bfloat16 over the scores in
-//                   tensor memory
+//   P = softmax(S)  a thread a row: mask, running maximum and sum in 32 bits, 2^x, P rounded to bfloat16 into tensor memory
 //   O += P V        P from tensor memory
-// O accumulates in tensor memory relative to a reference maximum and is rescaled only when a row's maximum has grown by more
-// than 2^8.  A group's scores follow its own P V in the tensor cores' queue, so scores that have arrived say that O is complete;
-// the groups take turns, one at its softmax while the products of the other run.
+// Two groups of four warps take the tiles in turn, even and odd ones, each a thread a row of the same 128 rows.  Tensor memory
+// holds two S, two P and the one O: the scores of a group's next tile are formed as soon as it has read the present ones, so
+// that no group waits for the tensor cores, and neither do they for a group.  (Two groups with rows, S, P over S and O of their
+// own instead: a tile of 128 keys and 256 rows took 4,450 cycles, of which 1,700 went into the signals between the warps
+// alone, and none of the ways to shorten them helped: 64 keys a tile, two threads a row, fewer registers.)
+// The groups share a row's reference maximum, to which O is relative: a group decides on it for its tile after the other has
+// for the tile before, which it learns through shared memory.  The reference follows the maximum only when that has grown by
+// more than 2^8, and O is then rescaled in place, the product of the tile before being complete.  Each group keeps a sum of its own.
 //
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
@@ -32,23 +36,24 @@ namespace {
 
 constexpr int D = LAB_HEAD_DIM;
 constexpr int KEYS = 128, ROWS = 128, GROUPS = 2, THREADS = 384;
-constexpr int STAGES = D == 64 ? 4 : 2;
+constexpr int STAGES = D == 64 ? 4 : 3;
 constexpr int HALVES = D / 64, HALF_BYTES = KEYS * 128;      // swizzled tiles of 64 columns, 128 bytes a row
 constexpr int TILE = HALVES * HALF_BYTES;                    // 128 rows
-constexpr int OFF_Q = 0;                                     // [group]
-constexpr int OFF_K = OFF_Q + GROUPS * TILE;
+constexpr int OFF_Q = 0;
+constexpr int OFF_K = OFF_Q + TILE;
 constexpr int OFF_V = OFF_K + STAGES * TILE;
-constexpr int OFF_BAR = OFF_V + STAGES * TILE;
+constexpr int OFF_ROW = OFF_V + STAGES * TILE;               // a row's reference maximum, and its two sums
+constexpr int OFF_BAR = OFF_ROW + 3 * ROWS * 4;
 constexpr int SMEM = OFF_BAR + 384 + 1024;
 static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
-constexpr int TM_S = 0, TM_O = GROUPS * KEYS, TMEM_COLS = 512;
-static_assert(TM_O + GROUPS * D <= TMEM_COLS, "tensor memory holds two S and two O");
+constexpr int TM_S = 0, TM_P = GROUPS * KEYS, TM_O = TM_P + GROUPS * KEYS / 2, TMEM_COLS = 512;
+static_assert(TM_O + D <= TMEM_COLS, "tensor memory holds two S, two P and one O");
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE = 8.f;
 
 struct Barriers {
-  uint64_t q_full[GROUPS], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[GROUPS], p_full[GROUPS], o_full[GROUPS],
-      turn[GROUPS][4];
+  uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[GROUPS], s_empty[GROUPS], p_full[GROUPS],
+      o_full[GROUPS], turn[GROUPS][4];
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -153,14 +158,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   // kv heads fastest, a request's last rows first: the CTAs that walk the most keys start in the first wave
   const int b = blockIdx.z, kvh = blockIdx.x, group = a.n_q / a.n_kv;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
-  const int r0 = (gridDim.y - 1 - blockIdx.y) * (GROUPS * ROWS);
+  const int r0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
   if (ql < a.fewest || r0 >= ql * group) {
     pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
     return;
   }
   const int p0 = a.pos0[b];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int last_row = min(r0 + GROUPS * ROWS, ql * group) - 1;
+  const int last_row = min(r0 + ROWS, ql * group) - 1;
   const int pos_lo = p0 + r0 / group, pos_hi = p0 + last_row / group;
   const int last = min(min(pos_hi, a.kv_len[b] - 1), a.max_blocks * a.page_size - 1), first = lab_first_key(pos_lo, a.window);
   const int t_lo = first / KEYS, n_tiles = last >= first ? last / KEYS - t_lo + 1 : 0;
@@ -172,9 +177,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       mbar_init(&bar->v_full[s], 1);
       mbar_init(&bar->v_empty[s], 1);
     }
+    mbar_init(&bar->q_full, 4);
     for (int g = 0; g < GROUPS; ++g) {
-      mbar_init(&bar->q_full[g], 4);
       mbar_init(&bar->s_full[g], 1);
+      mbar_init(&bar->s_empty[g], 4);
       mbar_init(&bar->p_full[g], 4);
       mbar_init(&bar->o_full[g], 1);
       for (int w = 0; w < 4; ++w) mbar_init(&bar->turn[g][w], 1);
@@ -222,69 +228,63 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       // ---------------- products ----------------
       constexpr uint32_t idesc_s = umma_instr_desc(ROWS, KEYS), idesc_o = umma_instr_desc(ROWS, D, true);
       auto wait_all = [&](uint64_t* m, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(m, parity, abort_flag)); };
-      auto issue_s = [&](int j, int g) {
+      auto issue_s = [&](int j) -> bool {      // into its group's buffer, which has been read
+        if (!wait_all(&bar->k_full[j % STAGES], (j / STAGES) & 1) || !wait_all(&bar->s_empty[j & 1], ((j >> 1) & 1) ^ 1)) return false;
+        tc_fence_after();
 #pragma unroll
         for (int hf = 0; hf < HALVES; ++hf) {
-          const uint64_t qd = smem_desc_sw128(smem_base + OFF_Q + g * TILE + hf * HALF_BYTES),
+          const uint64_t qd = smem_desc_sw128(smem_base + OFF_Q + hf * HALF_BYTES),
                          kd = smem_desc_sw128(smem_base + OFF_K + (j % STAGES) * TILE + hf * HALF_BYTES);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base + TM_S + g * KEYS, qd + 2 * k, kd + 2 * k, idesc_s, (hf | k) > 0);
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base + TM_S + (j & 1) * KEYS, qd + 2 * k, kd + 2 * k, idesc_s, (hf | k) > 0);
         }
-        umma_commit(&bar->s_full[g]);
+        umma_commit(&bar->s_full[j & 1]);
+        umma_commit(&bar->k_empty[j % STAGES]);
+        return true;
       };
-      bool ok = n_tiles > 0 && wait_all(&bar->k_full[0], 0);
-      for (int g = 0; g < GROUPS && ok; ++g) {
-        ok = wait_all(&bar->q_full[g], 0);
-        tc_fence_after();
-        if (ok) issue_s(0, g);
-      }
-      if (ok) umma_commit(&bar->k_empty[0]);
+      bool ok = n_tiles > 0 && wait_all(&bar->q_full, 0) && issue_s(0) && (n_tiles == 1 || issue_s(1));
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j % STAGES, next = (j + 1) % STAGES;
-        // (both are there long before the rows' P)
-        ok = wait_all(&bar->v_full[s], (j / STAGES) & 1);
-        if (ok && j + 1 < n_tiles) ok = wait_all(&bar->k_full[next], ((j + 1) / STAGES) & 1);
-        const uint64_t vd = q8_desc(smem_base + OFF_V + s * TILE, HALF_BYTES, 1024, 2);
-        for (int g = 0; g < GROUPS && ok; ++g) {
-          ok = wait_all(&bar->p_full[g], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < KEYS / 16; ++k)      // 16 keys of V lie 16 rows of 128 bytes on
-            umma_bf16_tmem_a(tmem_base + TM_O + g * D, tmem_base + TM_S + g * KEYS + k * 8, vd + (uint64_t)(k * 16 * 128 / 16), idesc_o,
-                             (k | j) > 0);
-          if (j + 1 < n_tiles) issue_s(j + 1, g);
-          else umma_commit(&bar->o_full[g]);
-        }
+        if (j + 2 < n_tiles && !issue_s(j + 2)) break;
+        const int s = j % STAGES;
+        ok = wait_all(&bar->v_full[s], (j / STAGES) & 1) && wait_all(&bar->p_full[j & 1], (j >> 1) & 1);
         if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = q8_desc(smem_base + OFF_V + s * TILE, HALF_BYTES, 1024, 2);
+#pragma unroll
+        for (int k = 0; k < KEYS / 16; ++k)      // 16 keys of V lie 16 rows of 128 bytes on
+          umma_bf16_tmem_a(tmem_base + TM_O, tmem_base + TM_P + (j & 1) * (KEYS / 2) + k * 8, vd + (uint64_t)(k * 16 * 128 / 16), idesc_o, (k | j) > 0);
+        umma_commit(&bar->o_full[j & 1]);
         umma_commit(&bar->v_empty[s]);
-        if (j + 1 < n_tiles) umma_commit(&bar->k_empty[next]);
       }
     }
   } else {
-    // ---------------- softmax: a thread a row ----------------
+    // ---------------- softmax: a thread a row, a group every other tile ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int g = (warp - 4) >> 2, quarter = warp & 3, mine = quarter * 32 + lane;
-    const int r = r0 + g * ROWS + mine, token = r / group, head = kvh * group + r - token * group;
+    const int r = r0 + mine, token = r / group, head = kvh * group + r - token * group;
     const bool valid = r < ql * group;
     const int pos = p0 + token, hi = valid ? min(pos, last) : -1, lo = lab_first_key(pos, a.window);
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    {
+    if (g == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(qs + token) * a.q_stride + (size_t)head * D);
-      uint8_t* q_s = smem + OFF_Q + g * TILE + mine * 128;
+      uint8_t* q_s = smem + OFF_Q + mine * 128;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
         *reinterpret_cast<uint4*>(q_s + (c >> 3) * HALF_BYTES + ((c & 7) ^ (mine & 7)) * 16) = valid ? src[c] : make_uint4(0, 0, 0, 0);
       proxy_fence();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->q_full[g]);
+      if (lane == 0) mbar_arrive(&bar->q_full);
     }
-    const uint32_t s_addr = lane_addr + TM_S + g * KEYS, o_addr = lane_addr + TM_O + g * D;
+    const uint32_t s_addr = lane_addr + TM_S + g * KEYS, p_addr = lane_addr + TM_P + g * (KEYS / 2), o_addr = lane_addr + TM_O;
     const f32x2 factor2 = pair_of(a.scale_log2, a.scale_log2);
+    volatile float* reference = reinterpret_cast<volatile float*>(smem + OFF_ROW) + mine;      // then the two sums, ROWS further each
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      ok = mbar_wait(&bar->s_full[g], j & 1, abort_flag);
+    // the other group's decision for tile j - 1 has been made
+    auto told = [&](int j) { return __all_sync(0xffffffffu, mbar_wait(&bar->turn[g][quarter], ((j - 1) >> 1) & 1, abort_flag)); };
+    for (int j = g; j < n_tiles; j += GROUPS) {
+      const uint32_t phase = (j >> 1) & 1;
+      ok = mbar_wait(&bar->s_full[g], phase, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -292,6 +292,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
 #pragma unroll
       for (int c = 0; c < KEYS / 32; ++c) tmem_ld32_issue(s_addr + c * 32, sr + c * 32);
       tmem_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->s_empty[g]);
       const int key0 = (t_lo + j) * KEYS;
       if (!__all_sync(0xffffffffu, key0 >= lo && key0 + KEYS - 1 <= hi)) {
         const int from = lo - key0, to = hi - key0;
@@ -302,11 +305,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < KEYS; c += 2) mx4[(c >> 1) & 3] = max_of(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-      const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2);
-      if (j == 0) {
-        m_ref = m_new;
-      } else if (__any_sync(0xffffffffu, m_new > m_ref + RESCALE || (m_ref == -INFINITY && m_new != -INFINITY))) {
-        const float f = m_ref == m_new ? 1.f : fast_exp2(m_ref - m_new);
+      const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+      float m_old = -INFINITY;
+      if (j > 0) {
+        ok = told(j);
+        if (!ok) break;
+        m_old = *reference;
+      }
+      const float m_top = fmaxf(m_old, top);
+      const bool grows = __any_sync(0xffffffffu, m_top > m_old + RESCALE || (m_old == -INFINITY && m_top != -INFINITY));
+      const float m_new = grows ? m_top : m_old;
+      *reference = m_new;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->turn[g ^ 1][quarter]);
+      l *= m_ref == m_new ? 1.f : fast_exp2(m_ref - m_new);
+      m_ref = m_new;
+      // this group's P of two tiles ago has been multiplied, and with it all before that
+      if (j >= GROUPS) {
+        ok = mbar_wait(&bar->o_full[g], phase ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      if (grows && j > 0) {
+        ok = mbar_wait(&bar->o_full[g ^ 1], ((j - 1) >> 1) & 1, abort_flag);      // and that of the tile before
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float f = m_old == m_new ? 1.f : fast_exp2(m_old - m_new);
 #pragma unroll
         for (int part = 0; part < D / 16; ++part) {
           uint32_t o[16];
@@ -316,16 +341,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
           for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
           tmem_st16(o_addr + part * 16, o);
         }
-        l *= f;
-        m_ref = m_new;
       }
       const float base = m_ref == -INFINITY ? 0.f : m_ref;
       const f32x2 base2 = pair_of(-base, -base);
-      // The groups take turns at their exponentials (a warp with the one of its scheduler): side by side they finish together,
-      // and the tensor cores then wait for both and both for them.
-      ok = mbar_wait(&bar->turn[g][quarter], g == 0 ? (j & 1) ^ 1 : j & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
       f32x2 sum2[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < KEYS / 32; ++c) {
@@ -337,9 +355,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
           sum2[i & 1] = add2(sum2[i & 1], pair_of(p, q));
           pk[i] = pack_bf16(p, q);
         }
-        tmem_st16(s_addr + c * 16, pk);
+        tmem_st16(p_addr + c * 16, pk);
       }
-      if (lane == 0) mbar_arrive(&bar->turn[g ^ 1][quarter]);
       const f32x2 sum = add2(sum2[0], sum2[1]);
       l += low_of(sum) + high_of(sum);
       tmem_st_wait();
@@ -347,18 +364,27 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->p_full[g]);
     }
+    // The row's sum: each group's, relative to the last reference.
     if (ok && n_tiles > 0) {
-      ok = mbar_wait(&bar->o_full[g], 0, abort_flag);
+      if (((n_tiles - 1) & 1) != g) ok = told(n_tiles);
+      const float m_last = *reference;
+      l *= m_ref == m_last ? 1.f : fast_exp2(m_ref - m_last);
+    }
+    reference[(1 + g) * ROWS] = l;
+    asm volatile("bar.sync 1, 256;" ::: "memory");      // (a group that has given up comes here too)
+    l += reference[(1 + (g ^ 1)) * ROWS];
+    if (ok && n_tiles > 0) {
+      ok = mbar_wait(&bar->o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok) {
+    if (ok) {      // half of the head's entries a group
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      __nv_bfloat16* dst = a.out + (size_t)(qs + token) * a.out_stride + (size_t)head * D;
+      __nv_bfloat16* dst = a.out + (size_t)(qs + token) * a.out_stride + (size_t)head * D + g * (D / 2);
 #pragma unroll
-      for (int part = 0; part < D / 32; ++part) {
+      for (int part = 0; part < D / 64; ++part) {
         uint32_t x[32];
-        tmem_ld32_issue(o_addr + part * 32, x);   // every lane takes part in the load
+        tmem_ld32_issue(o_addr + g * (D / 2) + part * 32, x);   // every lane takes part in the load
         tmem_wait();
         if (!valid) continue;
         auto number = [&](int i) { return n_tiles == 0 ? 0.f : __uint_as_float(x[i]) * inv; };
@@ -430,7 +456,7 @@ LAB_EXPORT int lab_attention_q8_rows(void* out, int out_stride, const void* q, l
   if (e != cudaSuccess) return (int)e;
   e = lab_launch(widen_kernel, dim3(span / KEYS, n_kv, requests), dim3(WIDEN_THREADS), 0, stream, a);
   if (e != cudaSuccess) return (int)e;
-  const long long tiles = ((long long)longest * (n_q / n_kv) + GROUPS * ROWS - 1) / (GROUPS * ROWS);
+  const long long tiles = ((long long)longest * (n_q / n_kv) + ROWS - 1) / ROWS;
   if (tiles > 65535) return (int)cudaErrorInvalidValue;
   return (int)lab_launch(attention_q8_rows_kernel, dim3(n_kv, (unsigned)tiles, requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
 }
