@@ -24,7 +24,7 @@
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
 //
-// Warps: 0 loads (TMA), 1 issues the products, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of 168 registers become 224
+// Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of 168 registers become 224
 // a softmax thread and 56 the rest: 2 x 224 + 56 = 3 x 168.  Every wait is bounded.
 #include "quant8_tc.cuh"
 
@@ -225,35 +225,37 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
         }
       }
     } else if (warp == 1) {
-      // ---------------- products ----------------
-      constexpr uint32_t idesc_s = umma_instr_desc(ROWS, KEYS), idesc_o = umma_instr_desc(ROWS, D, true);
-      auto wait_all = [&](uint64_t* m, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(m, parity, abort_flag)); };
-      auto issue_s = [&](int j) -> bool {      // into its group's buffer, which has been read
-        if (!wait_all(&bar->k_full[j % STAGES], (j / STAGES) & 1) || !wait_all(&bar->s_empty[j & 1], ((j >> 1) & 1) ^ 1)) return false;
+      // ---------------- scores: a group's next as soon as it has read the present ones ----------------
+      constexpr uint32_t idesc = umma_instr_desc(ROWS, KEYS);
+      bool ok = n_tiles > 0 && mbar_wait(&bar->q_full, 0, abort_flag);
+      for (int j = 0; j < n_tiles; ++j) {
+        const int s = j % STAGES, g = j & 1;
+        ok = ok && mbar_wait(&bar->k_full[s], (j / STAGES) & 1, abort_flag) && mbar_wait(&bar->s_empty[g], ((j >> 1) & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
 #pragma unroll
         for (int hf = 0; hf < HALVES; ++hf) {
-          const uint64_t qd = smem_desc_sw128(smem_base + OFF_Q + hf * HALF_BYTES),
-                         kd = smem_desc_sw128(smem_base + OFF_K + (j % STAGES) * TILE + hf * HALF_BYTES);
+          const uint64_t qd = smem_desc_sw128(smem_base + OFF_Q + hf * HALF_BYTES), kd = smem_desc_sw128(smem_base + OFF_K + s * TILE + hf * HALF_BYTES);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base + TM_S + (j & 1) * KEYS, qd + 2 * k, kd + 2 * k, idesc_s, (hf | k) > 0);
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base + TM_S + g * KEYS, qd + 2 * k, kd + 2 * k, idesc, (hf | k) > 0);
         }
-        umma_commit(&bar->s_full[j & 1]);
-        umma_commit(&bar->k_empty[j % STAGES]);
-        return true;
-      };
-      bool ok = n_tiles > 0 && wait_all(&bar->q_full, 0) && issue_s(0) && (n_tiles == 1 || issue_s(1));
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        if (j + 2 < n_tiles && !issue_s(j + 2)) break;
-        const int s = j % STAGES;
-        ok = wait_all(&bar->v_full[s], (j / STAGES) & 1) && wait_all(&bar->p_full[j & 1], (j >> 1) & 1);
-        if (!ok) break;
+        umma_commit(&bar->s_full[g]);
+        umma_commit(&bar->k_empty[s]);
+      }
+    } else if (warp == 2) {
+      // ---------------- P V: as soon as P is there (a warp of its own: neither kind of product waits for the other's operands) ----------------
+      constexpr uint32_t idesc = umma_instr_desc(ROWS, D, true);
+      bool ok = true;
+      for (int j = 0; j < n_tiles; ++j) {
+        const int s = j % STAGES, g = j & 1;
+        ok = mbar_wait(&bar->v_full[s], (j / STAGES) & 1, abort_flag) && mbar_wait(&bar->p_full[g], (j >> 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint64_t vd = q8_desc(smem_base + OFF_V + s * TILE, HALF_BYTES, 1024, 2);
 #pragma unroll
         for (int k = 0; k < KEYS / 16; ++k)      // 16 keys of V lie 16 rows of 128 bytes on
-          umma_bf16_tmem_a(tmem_base + TM_O, tmem_base + TM_P + (j & 1) * (KEYS / 2) + k * 8, vd + (uint64_t)(k * 16 * 128 / 16), idesc_o, (k | j) > 0);
-        umma_commit(&bar->o_full[j & 1]);
+          umma_bf16_tmem_a(tmem_base + TM_O, tmem_base + TM_P + g * (KEYS / 2) + k * 8, vd + (uint64_t)(k * 16 * 128 / 16), idesc, (k | j) > 0);
+        umma_commit(&bar->o_full[g]);
         umma_commit(&bar->v_empty[s]);
       }
     }
@@ -280,8 +282,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     volatile float* reference = reinterpret_cast<volatile float*>(smem + OFF_ROW) + mine;      // then the two sums, ROWS further each
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
-    // the other group's decision for tile j - 1 has been made
-    auto told = [&](int j) { return __all_sync(0xffffffffu, mbar_wait(&bar->turn[g][quarter], ((j - 1) >> 1) & 1, abort_flag)); };
     for (int j = g; j < n_tiles; j += GROUPS) {
       const uint32_t phase = (j >> 1) & 1;
       ok = mbar_wait(&bar->s_full[g], phase, abort_flag);
@@ -295,6 +295,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->s_empty[g]);
+      // Two conditions that hold by now as a rule are asked for here and looked at when they are needed: the other group has
+      // decided for the tile before, and this group's P of two tiles ago has been multiplied (and with it all before that).
+      const bool decided = j == 0 || mbar_try_wait(&bar->turn[g][quarter], ((j - 1) >> 1) & 1);
+      const bool multiplied = j < GROUPS || mbar_try_wait(&bar->o_full[g], phase ^ 1);
       const int key0 = (t_lo + j) * KEYS;
       if (!__all_sync(0xffffffffu, key0 >= lo && key0 + KEYS - 1 <= hi)) {
         const int from = lo - key0, to = hi - key0;
@@ -307,11 +311,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       for (int c = 0; c < KEYS; c += 2) mx4[(c >> 1) & 3] = max_of(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
       const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
       float m_old = -INFINITY;
-      if (j > 0) {
-        ok = told(j);
-        if (!ok) break;
-        m_old = *reference;
+      if (!__all_sync(0xffffffffu, decided && multiplied)) {
+        if (!decided) ok = mbar_wait(&bar->turn[g][quarter], ((j - 1) >> 1) & 1, abort_flag);
+        if (!multiplied) ok = mbar_wait(&bar->o_full[g], phase ^ 1, abort_flag) && ok;
+        if (!__all_sync(0xffffffffu, ok)) break;
       }
+      if (j > 0) m_old = *reference;
       const float m_top = fmaxf(m_old, top);
       const bool grows = __any_sync(0xffffffffu, m_top > m_old + RESCALE || (m_old == -INFINITY && m_top != -INFINITY));
       const float m_new = grows ? m_top : m_old;
@@ -320,12 +325,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       if (lane == 0) mbar_arrive(&bar->turn[g ^ 1][quarter]);
       l *= m_ref == m_new ? 1.f : fast_exp2(m_ref - m_new);
       m_ref = m_new;
-      // this group's P of two tiles ago has been multiplied, and with it all before that
-      if (j >= GROUPS) {
-        ok = mbar_wait(&bar->o_full[g], phase ^ 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
       if (grows && j > 0) {
         ok = mbar_wait(&bar->o_full[g ^ 1], ((j - 1) >> 1) & 1, abort_flag);      // and that of the tile before
         ok = __all_sync(0xffffffffu, ok);
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     }
     // The row's sum: each group's, relative to the last reference.
     if (ok && n_tiles > 0) {
-      if (((n_tiles - 1) & 1) != g) ok = told(n_tiles);
+      if (((n_tiles - 1) & 1) != g) ok = mbar_wait(&bar->turn[g][quarter], ((n_tiles - 1) >> 1) & 1, abort_flag);
       const float m_last = *reference;
       l *= m_ref == m_last ? 1.f : fast_exp2(m_ref - m_last);
     }
