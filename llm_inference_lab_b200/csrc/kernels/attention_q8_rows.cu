@@ -102,24 +102,31 @@ __global__ void __launch_bounds__(WIDEN_THREADS) widen_kernel(const Args a) {
     return;
   }
   const size_t to0 = (((size_t)place * a.n_kv + kvh) * a.span + (size_t)blockIdx.x * KEYS) * D;
-  constexpr int PIECES = D / 16;
-  for (int e = threadIdx.x; e < KEYS * PIECES; e += WIDEN_THREADS) {
-    const int row = e / PIECES, piece = e % PIECES, j = key0 + row;
-    uint4 kc = make_uint4(0, 0, 0, 0), vc = kc;
-    float ks = 0.f, vs = 0.f;
-    if (j >= first && j <= last) {
-      const int page = bt[j / a.page_size];
-      if (page < 0 || page >= a.num_pages) {      // a page that holds visible keys must exist
-        lab_set_error(LAB_ERR_PAGE_RANGE);
-      } else {
-        const size_t at = ((size_t)page * a.n_kv + kvh) * a.page_size + j % a.page_size;
-        kc = *reinterpret_cast<const uint4*>(a.k + at * D + piece * 16);
-        vc = *reinterpret_cast<const uint4*>(a.v + at * D + piece * 16);
-        const uint32_t kb = a.k_scale[at], vb = a.v_scale[at];
-        ks = q8_scale(vb == Q8_NAN_BYTE ? Q8_NAN_BYTE : kb);
-        vs = vb == Q8_NAN_BYTE ? 0.f : q8_scale(vb);
-      }
+  constexpr int PIECES = D / 16, TURNS = KEYS * PIECES / WIDEN_THREADS;
+  static_assert(KEYS * PIECES % WIDEN_THREADS == 0, "whole turns");
+  uint4 kc[TURNS], vc[TURNS];
+  float ks[TURNS], vs[TURNS];
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) {      // all loads of a thread in flight together
+    const int e = t * WIDEN_THREADS + threadIdx.x, j = key0 + e / PIECES, piece = e % PIECES;
+    kc[t] = vc[t] = make_uint4(0, 0, 0, 0);
+    ks[t] = vs[t] = 0.f;
+    if (j < first || j > last) continue;
+    const int page = bt[j / a.page_size];
+    if (page < 0 || page >= a.num_pages) {      // a page that holds visible keys must exist
+      lab_set_error(LAB_ERR_PAGE_RANGE);
+      continue;
     }
+    const size_t at = ((size_t)page * a.n_kv + kvh) * a.page_size + j % a.page_size;
+    kc[t] = *reinterpret_cast<const uint4*>(a.k + at * D + piece * 16);
+    vc[t] = *reinterpret_cast<const uint4*>(a.v + at * D + piece * 16);
+    const uint32_t kb = a.k_scale[at], vb = a.v_scale[at];
+    ks[t] = q8_scale(vb == Q8_NAN_BYTE ? Q8_NAN_BYTE : kb);
+    vs[t] = vb == Q8_NAN_BYTE ? 0.f : q8_scale(vb);
+  }
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) {
+    const int e = t * WIDEN_THREADS + threadIdx.x;
     auto put = [&](__nv_bfloat16* out, const uint4& c, float f) {
       const uint32_t w[4] = {c.x, c.y, c.z, c.w};
       uint32_t r[8];
@@ -128,12 +135,12 @@ __global__ void __launch_bounds__(WIDEN_THREADS) widen_kernel(const Args a) {
         const float4 x = q8_decode4(w[i]);
         r[2 * i] = pack_bf16(x.x * f, x.y * f), r[2 * i + 1] = pack_bf16(x.z * f, x.w * f);
       }
-      uint4* to = reinterpret_cast<uint4*>(out + to0 + (size_t)row * D + piece * 16);
+      uint4* to = reinterpret_cast<uint4*>(out + to0 + (size_t)(e / PIECES) * D + (e % PIECES) * 16);
       to[0] = make_uint4(r[0], r[1], r[2], r[3]);
       to[1] = make_uint4(r[4], r[5], r[6], r[7]);
     };
-    put(a.wide_k, kc, ks);
-    put(a.wide_v, vc, vs);
+    put(a.wide_k, kc[t], ks[t]);
+    put(a.wide_v, vc[t], vs[t]);
   }
 }
 
