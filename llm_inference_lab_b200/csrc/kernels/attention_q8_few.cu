@@ -30,7 +30,7 @@ constexpr int D = LAB_HEAD_DIM;
 using Tile = Q8Tile<D>;
 constexpr int KEYS = Tile::KEYS;
 constexpr int THREADS = 192;
-constexpr int STAGES = D == 64 ? 4 : 3;
+constexpr int STAGES = D == 64 ? 4 : 2;
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int N> struct Layout {
@@ -69,7 +69,7 @@ struct Args {
 };
 
 template <int N>
-__global__ void __launch_bounds__(THREADS, N <= 32 ? 2 : 1) attention_q8_few_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attention_q8_few_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const Args a) {
   using L = Layout<N>;
   extern __shared__ uint8_t smem_raw[];

@@ -129,13 +129,12 @@ template <typename T, bool PARTS, int N>
 __global__ void __launch_bounds__(PARTS ? FEW_THREADS : THREADS) store_vec_kernel(const Store s) {
   pdl_trigger();
   pdl_wait();
-  const int lanes = s.d / (2 * N), half = s.d / 2, heads = s.n_q + 2 * s.n_kv;
-  const long long unit = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long row = unit / lanes;
-  if ((unit & ~31LL) / lanes >= (long long)s.tokens * heads) return;      // the whole warp
-  const bool there = row < (long long)s.tokens * heads;
-  const int token = there ? (int)(row / heads) : s.tokens - 1, head = there ? (int)(row - (long long)token * heads) : heads - 1;
-  const int at = (int)(unit % lanes) * N;
+  const int half = s.d / 2, lanes = half / N, shift = __ffs(lanes) - 1, heads = s.n_q + 2 * s.n_kv;
+  const unsigned unit = blockIdx.x * blockDim.x + threadIdx.x, row = unit >> shift, rows = (unsigned)s.tokens * heads;      // (the host checks: below 2^31)
+  if ((unit & ~31u) >> shift >= rows) return;      // the whole warp
+  const bool there = row < rows;
+  const int token = there ? (int)(row / heads) : s.tokens - 1, head = there ? (int)(row - token * heads) : heads - 1;
+  const int at = (int)(unit & (lanes - 1)) * N;
   float lo[N], hi[N];
   take<T, PARTS, N>(s, token, head * s.d + at, lo);
   take<T, PARTS, N>(s, token, head * s.d + at + half, hi);
@@ -253,45 +252,70 @@ int launch_store(const Store& s, bool vec, cudaStream_t stream) {
 }
 
 // ----------------------------------------------------------------------------------------
-// Reading back: a thread takes N codes of a key and leaves 16 bytes (N = 1: any size and alignment).
+// Reading back: a thread takes N codes of a key and of a value and leaves 16 bytes of each (N = 1: any size and alignment).
 // ----------------------------------------------------------------------------------------
-template <typename T, int N>
+// A thread keeps its place in the rows (so that what is divided is divided once) and takes EACH rows, their loads in flight together.
+template <typename T, int N, int EACH>
 __global__ void __launch_bounds__(THREADS) load_kernel(T* __restrict__ out_k, T* __restrict__ out_v, const uint8_t* __restrict__ k,
                                                        const uint8_t* __restrict__ v, const uint8_t* __restrict__ k_scale,
                                                        const uint8_t* __restrict__ v_scale, const int* __restrict__ slots, long long rows,
                                                        int n_kv, int d, int page_size, int num_pages) {
   pdl_trigger();
   pdl_wait();
-  const int pieces = d / N;
-  const long long unit = (long long)blockIdx.x * THREADS + threadIdx.x;
-  const long long head_row = unit / pieces;
-  if (head_row >= rows * n_kv) return;
-  const int at = (int)(unit - head_row * pieces) * N;
-  const long long row = head_row / n_kv;
-  const int head = (int)(head_row - row * n_kv), slot = slots[row];
-  const int page = slot >= 0 ? slot / page_size : -1;
-  if (page >= num_pages && at == 0) lab_set_error(LAB_ERR_PAGE_RANGE);
-  const bool held = page >= 0 && page < num_pages;
-  const long long place = held ? ((long long)page * n_kv + head) * page_size + (slot - page * page_size) : 0;
-  auto one = [&](T* out, const uint8_t* codes, const uint8_t* scales) {
-    const float f = held ? q8_scale(scales[place]) : 0.f;
-    T* to = out + head_row * d + at;
-    const uint8_t* from = codes + place * d + at;
+  // a block: EACH passes of as many whole rows as it has threads for, or of a piece of a row
+  const int pieces = d / N, width = n_kv * pieces, here = max(1, THREADS / width);
+  const int sub = threadIdx.x / width, place = blockIdx.y * THREADS + (here > 1 ? threadIdx.x - sub * width : threadIdx.x);
+  if (here > 1 ? sub >= here : place >= width) return;
+  const int head = place / pieces, at = (place - head * pieces) * N;
+  const long long row0 = (long long)blockIdx.x * here * EACH + (here > 1 ? sub : 0);
+  const int shift = (page_size & (page_size - 1)) == 0 ? __ffs(page_size) - 1 : -1;
+  long long from[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const long long row = row0 + i * here;
+    const int slot = row < rows ? slots[row] : -1;
+    const int page = slot < 0 ? -1 : shift >= 0 ? slot >> shift : slot / page_size;
+    if (page >= num_pages && at == 0) lab_set_error(LAB_ERR_PAGE_RANGE);
+    from[i] = page >= 0 && page < num_pages ? ((long long)page * n_kv + head) * page_size + (slot - page * page_size) : -1;
+  }
+  uint32_t kc[EACH][2], vc[EACH][2];
+  float kf[EACH], vf[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    kc[i][0] = kc[i][1] = vc[i][0] = vc[i][1] = 0u;
+    kf[i] = vf[i] = 0.f;
+    if (from[i] < 0) continue;
+    const uint8_t *kr = k + from[i] * d + at, *vr = v + from[i] * d + at;
     if constexpr (N == 8) {
-      const uint2 c = held ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
-      const float4 a = q8_decode4(c.x), b = q8_decode4(c.y);
-      const float x[8] = {a.x * f, a.y * f, a.z * f, a.w * f, b.x * f, b.y * f, b.z * f, b.w * f};
-      put<8>(to, x);
+      const uint2 x = *reinterpret_cast<const uint2*>(kr), y = *reinterpret_cast<const uint2*>(vr);
+      kc[i][0] = x.x, kc[i][1] = x.y, vc[i][0] = y.x, vc[i][1] = y.y;
     } else if constexpr (N == 4) {
-      const uint32_t c = held ? *reinterpret_cast<const uint32_t*>(from) : 0u;
-      const float4 a = q8_decode4(c);
-      store4(to, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
+      kc[i][0] = *reinterpret_cast<const uint32_t*>(kr), vc[i][0] = *reinterpret_cast<const uint32_t*>(vr);
     } else {
-      to[0] = from_f32<T>(held ? q8_decode(from[0]) * f : 0.f);
+      kc[i][0] = *kr, vc[i][0] = *vr;
     }
-  };
-  one(out_k, k, k_scale);
-  one(out_v, v, v_scale);
+    kf[i] = q8_scale(k_scale[from[i]]), vf[i] = q8_scale(v_scale[from[i]]);
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const long long row = row0 + i * here;
+    if (row >= rows) continue;
+    const size_t to = ((size_t)row * n_kv + head) * d + at;
+    auto one = [&](T* out, const uint32_t (&c)[2], float f) {
+      const float4 x = q8_decode4(c[0]);
+      if constexpr (N == 8) {
+        const float4 y = q8_decode4(c[1]);
+        const float z[8] = {x.x * f, x.y * f, x.z * f, x.w * f, y.x * f, y.y * f, y.z * f, y.w * f};
+        put<8>(out + to, z);
+      } else if constexpr (N == 4) {
+        store4(out + to, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+      } else {
+        out[to] = from_f32<T>(x.x * f);
+      }
+    };
+    one(out_k, kc[i], kf[i]);
+    one(out_v, vc[i], vf[i]);
+  }
 }
 
 template <typename T>
@@ -299,10 +323,16 @@ int launch_load(T* out_k, T* out_v, const uint8_t* k, const uint8_t* v, const ui
                 long long rows, int n_kv, int d, int page_size, int num_pages, cudaStream_t stream) {
   constexpr int N = 16 / sizeof(T);
   const bool vec = d % N == 0 && ((((uintptr_t)out_k) | ((uintptr_t)out_v)) & 15) == 0 && ((((uintptr_t)k) | ((uintptr_t)v)) & (N - 1)) == 0;
-  const long long units = rows * n_kv * (vec ? d / N : d);
-  const dim3 grid((unsigned)((units + THREADS - 1) / THREADS));
-  return (int)lab_launch(vec ? load_kernel<T, N> : load_kernel<T, 1>, grid, dim3(THREADS), 0, stream, out_k, out_v, k, v, k_scale, v_scale,
-                         slots, rows, n_kv, d, page_size, num_pages);
+  const long long width = (long long)n_kv * (vec ? d / N : d), here = width < THREADS ? THREADS / width : 1;
+  const long long across = (width + THREADS - 1) / THREADS;
+  // four rows a thread once every multiprocessor has two blocks of them (517 rows of 2 heads of 64, to bfloat16: 2.3 us by one
+  // row a thread, 4.4 by four; 40,000 rows of 4 heads of 128, to 32 bits: 56 and 40)
+  const bool four = rows / (here * 4) * across >= 2 * lab_sm_count();
+  const long long blocks = (rows + here * (four ? 4 : 1) - 1) / (here * (four ? 4 : 1));
+  if (blocks >= (1ll << 31) || across > 65535) return (int)cudaErrorInvalidValue;
+  return (int)lab_launch(vec ? four ? load_kernel<T, N, 4> : load_kernel<T, N, 1> : four ? load_kernel<T, 1, 4> : load_kernel<T, 1, 1>,
+                         dim3((unsigned)blocks, (unsigned)across), dim3(THREADS), 0, stream, out_k, out_v, k, v, k_scale, v_scale, slots, rows,
+                         n_kv, d, page_size, num_pages);
 }
 
 }  // namespace
@@ -318,7 +348,7 @@ LAB_EXPORT int lab_rope_kv_store_q8(const void* rows, long long row_stride, int 
                                     cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (d < 1 || d > MOST_DIM || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > d || n_q < 0 || n_kv < 1 || page_size < 1 || num_pages < 0 ||
-      parts < 0 || (parts > 0 && dtype != LAB_BF16) || (rotary_dim > 0 && table == nullptr))
+      (long long)tokens * (n_q + 2 * n_kv) * 32 >= (1ll << 31) || parts < 0 || (parts > 0 && dtype != LAB_BF16) || (rotary_dim > 0 && table == nullptr))
     return (int)cudaErrorInvalidValue;
   Store s;
   s.rows = rows, s.row_stride = row_stride, s.parts = parts, s.part_stride = part_stride, s.bias = (const __nv_bfloat16*)bias;

@@ -12,7 +12,7 @@
 // exact arithmetic only where two numbers agree to about 2^-20.
 //
 // Two launches: the rows' largest entry and sum of exponentials by chunk (every logit read once: the bound, memory), then a
-// cluster of eight CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that is
+// cluster of sixteen CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that is
 // left (its logits come from L2).  Partial results lie in the caller's scratch and nothing has to be zero before a call, so calls
 // on several streams, or from several graphs, do not meet.
 #include <limits.h>
@@ -21,7 +21,7 @@
 
 namespace {
 
-constexpr int CHUNK = 8192, STAT_THREADS = 256, PICK_THREADS = 512, CLUSTER = 8;
+constexpr int CHUNK = 8192, STAT_THREADS = 256, PICK_THREADS = 512, CLUSTER = 16, KEPT = 16;
 constexpr int ROUNDS = CHUNK / (STAT_THREADS * 4);
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
@@ -49,29 +49,12 @@ struct Args {
   int *tokens, *counts;
 };
 
-// A request's rows, none where `starts` is not ascending within the logits.
-__device__ __forceinline__ int2 rows_of(const Args& a, int b) {
-  const int lo = a.starts[b], hi = a.starts[b + 1];
-  return lo < 0 || hi > a.rows || hi < lo ? make_int2(0, 0) : make_int2(lo, hi);
-}
-
 __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args a) {
   __shared__ float sm[STAT_THREADS / 32], ss[STAT_THREADS / 32];
   __shared__ int si[STAT_THREADS / 32];
   pdl_trigger();
   pdl_wait();
   const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float inverse = 0.f;
-  if (a.temperature != nullptr) {
-    int b = 0, past = a.requests;
-    while (past - b > 1) {
-      const int mid = (b + past) / 2;
-      if (a.starts[mid] <= row) b = mid; else past = mid;
-    }
-    const float t = a.temperature[b];
-    inverse = t > 0.f ? 1.f / t : 0.f;
-  }
-  const bool greedy = inverse == 0.f;
   const float* lr = a.logits + (size_t)row * a.ld;
   const int first = chunk * CHUNK, end = min(a.vocab, first + CHUNK);
   float x[4 * ROUNDS];
@@ -87,6 +70,18 @@ __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args 
       for (int e = 0; e < 4; ++e) x[4 * r + e] = i + e < end ? lr[i + e] : __uint_as_float(0x7fffffffu);
     }
   }
+  // the row's request, looked for while its entries arrive
+  float inverse = 0.f;
+  if (a.temperature != nullptr) {
+    int b = 0, past = a.requests;
+    while (past - b > 1) {
+      const int mid = (b + past) / 2;
+      if (a.starts[mid] <= row) b = mid; else past = mid;
+    }
+    const float t = a.temperature[b];
+    inverse = t > 0.f ? 1.f / t : 0.f;
+  }
+  const bool greedy = inverse == 0.f;
   float m = -INFINITY;
   int at = INT_MAX;
   if (greedy) {
@@ -160,66 +155,95 @@ struct Best {
 };
 
 __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a, int cluster) {
-  __shared__ int stop_s, greedy_s;
-  __shared__ float m_s, inverse_sum_s;
+  __shared__ int stop_s;
+  __shared__ float4 stats_s[KEPT + 1];      // the first rows' statistics, and those of the row that ends the request
   __shared__ Best warp_s[PICK_THREADS / 32];
   __shared__ Best cta_s[CLUSTER];
   pdl_trigger();
   if (cluster > 1) cluster_sync();      // every CTA is there before another writes to it
   pdl_wait();
   const int b = blockIdx.x / cluster, part = blockIdx.x - b * cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int2 span = rows_of(a, b);
-  const int n = span.y - span.x;
-  const float t = a.temperature != nullptr ? a.temperature[b] : 0.f, inverse = t > 0.f ? 1.f / t : 0.f;
+  // what a request has one of, asked for together
+  const int lo = a.starts[b], hi = a.starts[b + 1];
+  const float t = a.temperature != nullptr ? a.temperature[b] : 0.f;
+  const uint32_t seed = a.temperature != nullptr ? a.seeds[b] : 0u;
+  const int position = a.temperature != nullptr ? a.positions[b] : 0;
+  const bool sound = lo >= 0 && hi <= a.rows && hi >= lo;      // rows ascending within the logits
+  const int n = sound ? hi - lo : 0;
+  const float inverse = t > 0.f ? 1.f / t : 0.f;
   const bool greedy = inverse == 0.f;
   if (threadIdx.x == 0) {
     stop_s = max(n - 1, 0);
-    if (part == 0 && (a.starts[b] < 0 || a.starts[b + 1] > a.rows || a.starts[b + 1] < a.starts[b])) lab_set_error(LAB_ERR_ROW_RANGE);
+    if (part == 0 && !sound) lab_set_error(LAB_ERR_ROW_RANGE);
   }
   __syncthreads();
-  auto key_of = [&](int i) { return mix32(mix32(a.seeds[b] ^ 0x9E3779B9u) ^ (uint32_t)(a.positions[b] + i)); };
-  for (int i = warp; i < n - 1; i += PICK_THREADS / 32) {
-    const int row = span.x + i, x = a.drafts[row];
+  auto key_of = [&](int i) { return mix32(mix32(seed ^ 0x9E3779B9u) ^ (uint32_t)(position + i)); };
+  for (int i = warp; i < n; i += PICK_THREADS / 32) {
+    const int row = lo + i, x = a.drafts[row];
+    const bool judged = i < n - 1, token = x >= 0 && x < a.vocab, gathers = judged && token && !greedy;
+    const float logit = gathers ? a.logits[(size_t)row * a.ld + x] : 0.f;
+    const float q = gathers && a.draft_probs != nullptr ? a.draft_probs[(size_t)row * a.ld_probs + x] : 1.f;
     const float4 s = row_stats(a, row, lane);
-    bool taken = x >= 0 && x < a.vocab;
+    bool taken = token;
     if (greedy) {
       taken = taken && x == __float_as_int(s.z);
     } else if (taken) {
-      const float v = a.logits[(size_t)row * a.ld + x] * inverse;
+      const float v = logit * inverse;
       const float p = (v == s.x ? 1.f : expf(v - s.x)) / s.y;
-      const float q = a.draft_probs != nullptr ? a.draft_probs[(size_t)row * a.ld_probs + x] : 1.f;
       taken = uniform_of(mix32(~key_of(i))) * q < p;
     }
-    if (!taken && lane == 0) atomicMin(&stop_s, i);
+    if (lane == 0) {
+      if (judged && !taken) atomicMin(&stop_s, i);
+      if (i < KEPT) stats_s[i] = s;
+    }
   }
   __syncthreads();
-  const int stop = stop_s, row = span.x + stop;
-  if (warp == 0 && n > 0) {
-    const float4 s = row_stats(a, row, lane);
-    if (lane == 0) m_s = s.x, inverse_sum_s = 1.f / s.y, greedy_s = __float_as_int(s.z);
+  const int stop = stop_s, row = lo + stop;
+  if (stop >= KEPT) {      // (a request of many drafts)
+    if (warp == 0) {
+      const float4 s = row_stats(a, row, lane);
+      if (lane == 0) stats_s[KEPT] = s;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  const float4 ends = stats_s[min(stop, KEPT)];
   Best best = {0.f, 0.f, INT_MAX, INT_MAX};      // a weight above 0 is wanted
   if (!greedy && n > 0) {
-    const float m = m_s, inverse_sum = inverse_sum_s;
+    const float m = ends.x, inverse_sum = 1.f / ends.y;
     const uint32_t key = key_of(stop);
     const float* lr = a.logits + (size_t)row * a.ld;
     const bool over = stop == n - 1;
     const float* qr = !over && a.draft_probs != nullptr ? a.draft_probs + (size_t)row * a.ld_probs : nullptr;
     const int certain = !over && a.draft_probs == nullptr ? a.drafts[row] : -1;
+    // w / E <= w / (1 - u), so most entries are passed over without a logarithm: those that cannot beat what the warp has found.
+    float least = 0.f, p_least = 0.f;
     auto consider = [&](float logit, float q, int i) {
       const float v = logit * inverse;
-      const float p = (v == m ? 1.f : expf(v - m)) * inverse_sum;
+      const float p = (v == m ? 1.f : __expf(v - m)) * inverse_sum;
       const float w = i == certain ? 0.f : fmaxf(p - q, 0.f);
-      const float rate = __fdividef(1.f, -logf(uniform_of(mix32(key + (uint32_t)i * 0x85EBCA6Bu))));
-      if (better(w * rate, i, best.v, best.i)) best.v = w * rate, best.i = i;
-      if (better(p * rate, i, best.pv, best.pi)) best.pv = p * rate, best.pi = i;
+      const uint32_t h = mix32(key + (uint32_t)i * 0x85EBCA6Bu) >> 9;
+      const float rest = (8388607.5f - (float)h) * (1.f / 8388608.f);      // 1 - u
+      if (w >= least * rest || p >= p_least * rest) {
+        const float rate = __fdividef(1.f, -logf(((float)h + 0.5f) * (1.f / 8388608.f)));
+        if (better(w * rate, i, best.v, best.i)) best.v = w * rate, best.i = i;
+        if (better(p * rate, i, best.pv, best.pi)) best.pv = p * rate, best.pi = i;
+      }
     };
     const bool vec = (a.ld & 3) == 0 && (((uintptr_t)a.logits) & 15) == 0 &&
                      (qr == nullptr || ((a.ld_probs & 3) == 0 && (((uintptr_t)a.draft_probs) & 15) == 0));
-    for (int i = (part * PICK_THREADS + (int)threadIdx.x) * 4; i < a.vocab; i += cluster * PICK_THREADS * 4) {
+    const int step = cluster * PICK_THREADS * 4;
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto ask = [&](int i, float4& v, float4& q) {
+      const bool whole = vec && i + 3 < a.vocab;
+      v = whole ? load4(lr + i) : none;
+      q = whole && qr != nullptr ? load4(qr + i) : none;
+    };
+    float4 v, q, v_next, q_next;
+    ask(part * PICK_THREADS * 4 + (int)threadIdx.x * 4, v, q);
+    for (int base = part * PICK_THREADS * 4; base < a.vocab; base += step) {
+      const int i = base + (int)threadIdx.x * 4;
+      ask(i + step, v_next, q_next);
       if (vec && i + 3 < a.vocab) {
-        const float4 v = load4(lr + i), q = qr != nullptr ? load4(qr + i) : make_float4(0.f, 0.f, 0.f, 0.f);
         consider(v.x, q.x, i);
         consider(v.y, q.y, i + 1);
         consider(v.z, q.z, i + 2);
@@ -227,6 +251,10 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a,
       } else {
         for (int e = i; e < min(i + 4, a.vocab); ++e) consider(lr[e], qr != nullptr ? qr[e] : 0.f, e);
       }
+      v = v_next, q = q_next;
+      // a little less than the best: what the bound's own rounding could lose
+      least = warp_max(best.v) * 0.9999f;
+      p_least = warp_max(best.pv) * 0.9999f;
     }
   }
   auto over_lanes = [&]() {
@@ -263,9 +291,9 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a,
     return;
   }
   for (int i = threadIdx.x; i < n; i += PICK_THREADS)
-    if (i != stop) a.tokens[span.x + i] = i < stop ? a.drafts[span.x + i] : -1;
+    if (i != stop) a.tokens[lo + i] = i < stop ? a.drafts[lo + i] : -1;
   if (threadIdx.x == 0) {
-    a.tokens[row] = greedy ? greedy_s : best.v > 0.f ? best.i : best.pi;
+    a.tokens[row] = greedy ? __float_as_int(ends.z) : best.v > 0.f ? best.i : best.pi;
     a.counts[b] = stop + 1;
   }
 }
@@ -294,7 +322,17 @@ LAB_EXPORT int lab_verify_drafts(int* tokens, int* counts, const float* logits, 
     const cudaError_t e = lab_launch(verify_chunks_kernel, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
     if (e != cudaSuccess) return (int)e;
   }
+  // a cluster beyond the portable size: asked for once per device
   const int cluster = temperature != nullptr ? CLUSTER : 1;
+  static std::atomic<bool> allowed[LabShared::kDevices] = {};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return (int)e;
+  if (device >= LabShared::kDevices || !allowed[device].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(verify_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return (int)e;
+    if (device < LabShared::kDevices) allowed[device].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(requests * cluster);
   cfg.blockDim = dim3(PICK_THREADS);

@@ -2448,7 +2448,7 @@ def q8_few_width(rows: int) -> int:
 
 def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
     """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once."""
-    room = (2 if width <= 32 else 1) * sm_count()
+    room = (3 if width <= 16 else 2 if width <= 32 else 1) * sm_count()
     return max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
 
 
