@@ -16,7 +16,7 @@ constexpr int WARPS = 4, MOST_DIM = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * WARPS) attention_q8_any_kernel(
-    T* __restrict__ out, int out_stride, const T* __restrict__ q, long long q_stride, const uint8_t* __restrict__ k,
+    T* __restrict__ out, long long out_stride, const T* __restrict__ q, long long q_stride, const uint8_t* __restrict__ k,
     const uint8_t* __restrict__ v, const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
     const int* __restrict__ q_start, const int* __restrict__ kv_len, const int* __restrict__ pos0, const int* __restrict__ block_table,
     int max_blocks, int requests, int n_q, int n_kv, int d, int page_size, int num_pages, int window, float scale) {
@@ -111,20 +111,27 @@ __global__ void __launch_bounds__(32 * WARPS) attention_q8_any_kernel(
 
 LAB_EXPORT int lab_attention_q8_most_dim() { return MOST_DIM; }
 
-// q: `tokens` rows q_stride elements apart, out likewise out_stride; both of `dtype`.  window as lab_first_key takes it.
-LAB_EXPORT int lab_attention_q8_any(void* out, int out_stride, const void* q, long long q_stride, int tokens, const void* k, const void* v,
-                                    const void* k_scale, const void* v_scale, const int* q_start, const int* kv_len, const int* pos0,
-                                    const int* block_table, int max_blocks, int requests, int n_q, int n_kv, int d, int page_size,
-                                    int num_pages, int window, float scale, int dtype, cudaStream_t stream) {
-  if (tokens <= 0 || requests <= 0) return 0;
-  if (d < 1 || d > MOST_DIM || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q > 65535 || page_size < 1 || num_pages < 0 || max_blocks < 0)
+// A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise, both of `dtype`.  window as lab_first_key
+// takes it.
+struct LabQ8Any {
+  void* out;
+  const void *q, *k, *v, *k_scale, *v_scale;
+  const int *q_start, *kv_len, *pos0, *block_table;
+  long long out_stride, q_stride;
+  int tokens, max_blocks, requests, n_q, n_kv, d, page_size, num_pages, window, dtype;
+  float scale;
+};
+
+LAB_EXPORT int lab_attention_q8_any(const LabQ8Any* c, cudaStream_t stream) {
+  if (c->tokens <= 0 || c->requests <= 0) return 0;
+  if (c->d < 1 || c->d > MOST_DIM || c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->n_q > 65535 || c->page_size < 1 || c->num_pages < 0 ||
+      c->max_blocks < 0)
     return (int)cudaErrorInvalidValue;
-  const dim3 grid(tokens, n_q);
   auto launch = [&](auto kernel, auto* o, auto* x) {
-    return (int)lab_launch(kernel, grid, dim3(32 * WARPS), 0, stream, o, out_stride, x, q_stride, (const uint8_t*)k, (const uint8_t*)v,
-                           (const uint8_t*)k_scale, (const uint8_t*)v_scale, q_start, kv_len, pos0, block_table, max_blocks, requests, n_q,
-                           n_kv, d, page_size, num_pages, window, scale);
+    return (int)lab_launch(kernel, dim3(c->tokens, c->n_q), dim3(32 * WARPS), 0, stream, o, c->out_stride, x, c->q_stride, (const uint8_t*)c->k,
+                           (const uint8_t*)c->v, (const uint8_t*)c->k_scale, (const uint8_t*)c->v_scale, c->q_start, c->kv_len, c->pos0,
+                           c->block_table, c->max_blocks, c->requests, c->n_q, c->n_kv, c->d, c->page_size, c->num_pages, c->window, c->scale);
   };
-  if (dtype == LAB_F32) return launch(attention_q8_any_kernel<float>, (float*)out, (const float*)q);
-  return launch(attention_q8_any_kernel<__nv_bfloat16>, (__nv_bfloat16*)out, (const __nv_bfloat16*)q);
+  if (c->dtype == LAB_F32) return launch(attention_q8_any_kernel<float>, (float*)c->out, (const float*)c->q);
+  return launch(attention_q8_any_kernel<__nv_bfloat16>, (__nv_bfloat16*)c->out, (const __nv_bfloat16*)c->q);
 }

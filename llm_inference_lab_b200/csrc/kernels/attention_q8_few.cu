@@ -17,7 +17,8 @@
 //
 // Warp 0 loads (TMA, a page a lane), warp 1 issues the products and owns tensor memory, warps 2-5 (128 threads) do the rest.
 // The scores of tile j + 1 are formed beside the softmax of tile j, and O^T of tile j - 1 beside it too.  The keys are split
-// over CTAs where there are fewer than the GPU holds, and merged by a second kernel.  Every wait is bounded.
+// over CTAs where there are fewer than the GPU holds, and merged inside a cluster of up to eight or by a second kernel.  Every wait
+// is bounded.
 #include "quant8_tc.cuh"
 
 #ifndef LAB_HEAD_DIM
@@ -63,10 +64,16 @@ struct Args {
   long long q_stride;
   const uint8_t *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  int max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, splits;
+  int max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, splits, cluster;
   float scale_log2;
   float *part_acc, *part_ml;
 };
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 template <int N>
 __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attention_q8_few_kernel(const __grid_constant__ CUtensorMap map_k,
@@ -431,6 +438,14 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     }
     asm volatile("bar.sync 2, 128;" ::: "memory");
     const int dim = D == 128 ? mine : quarter * 16 + lane;      // (64 rows of an accumulator: 16 lanes a quarter)
+    float* own = reinterpret_cast<float*>(smem + L::OFF_K);     // in a cluster: [N][D], then [N] references and [N] sums
+    if (a.cluster && w == 0) {
+      for (int n = lane; n < N; n += 32) {
+        const float4 s4 = load4(sums + n * 4);
+        own[N * D + n] = ok ? base_w[n] : -INFINITY;
+        own[N * D + N + n] = ok ? (s4.x + s4.y) + (s4.z + s4.w) : 0.f;
+      }
+    }
     if (ok && (D == 128 || lane < 16)) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -439,7 +454,9 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
         const float sum = (s4.x + s4.y) + (s4.z + s4.w);
         const int r = r0 + n, token = r / group, head = kvh * group + r - token * group;
         const float num = acc[n] * 0.00390625f;
-        if (a.splits == 1) {
+        if (a.cluster) {
+          own[n * D + dim] = num;
+        } else if (a.splits == 1) {
           a.out[(size_t)(qs + token) * a.out_stride + (size_t)head * D + dim] = __float2bfloat16_rn(sum == 0.f ? 0.f : num / sum);
         } else {
           const size_t slot = ((size_t)(qs + token) * a.n_q + head) * a.splits + split;
@@ -455,33 +472,81 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     tc_fence_after();
     tmem_dealloc(tmem_base, L::TMEM);
   }
+  if (a.cluster) {
+    // The splits of these rows are the cluster's CTAs: each merges every splits-th row out of the others' shared memory.
+    cluster_sync();
+    const uint32_t theirs = smem_base + L::OFF_K;
+    for (int e = threadIdx.x; e < N * D; e += THREADS) {
+      const int n = split + e / D * a.splits, dim = e % D;
+      if (n >= n_rows) break;
+      float acc[8], m[8], l[8], big = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t at = map_to_rank(theirs, i < a.splits ? i : 0);
+        acc[i] = ld_cluster_f32(at + (n * D + dim) * 4), m[i] = ld_cluster_f32(at + (N * D + n) * 4), l[i] = ld_cluster_f32(at + (N * D + N + n) * 4);
+        if (i >= a.splits) m[i] = -INFINITY, l[i] = 0.f, acc[i] = 0.f;
+        big = fmaxf(big, m[i]);
+      }
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - big);
+        num = fmaf(f, acc[i], num);
+        den = fmaf(f, l[i], den);      // (0 times a NaN is one: scores that are all none stay visible)
+      }
+      const int r = r0 + n, token = r / group, head = kvh * group + r - token * group;
+      a.out[(size_t)(qs + token) * a.out_stride + (size_t)head * D + dim] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+    }
+    cluster_sync();      // nobody's shared memory goes before the others have read it
+  }
 }
 
-// The splits of a row and query head put together: a block each, a thread an entry.
-__global__ void __launch_bounds__(D) attention_q8_merge_kernel(const Args a) {
+// The splits of a row and query head put together: a block each, a thread an entry, PARTS of them over the splits.
+constexpr int MERGE_PARTS = 1024 / 128;
+template <int PARTS>
+__global__ void __launch_bounds__(PARTS* D) attention_q8_merge_kernel(const Args a) {
+  __shared__ float num_s[PARTS][D], m_s[PARTS], den_s[PARTS];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, head = blockIdx.y, dim = threadIdx.x;
+  const int b = blockIdx.z, head = blockIdx.y, dim = threadIdx.x % D, part = threadIdx.x / D;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs, token = blockIdx.x;
   if (ql > a.most_rows || token >= ql) return;
   const size_t slot = ((size_t)(qs + token) * a.n_q + head) * a.splits;
-  float big = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) big = fmaxf(big, a.part_ml[(slot + s) * 2]);
-  float num = 0.f, den = 0.f;
-  for (int s0 = 0; s0 < a.splits; s0 += 8) {      // eight splits' loads in flight, added in their order
-    float acc[8], m[8], l[8];
+  const int each = (a.splits + PARTS - 1) / PARTS, end = min(a.splits, (part + 1) * each);
+  float big = -INFINITY, num = 0.f, den = 0.f;
+  for (int s0 = part * each; s0 < end; s0 += 8) {      // eight splits' loads in flight, added in their order
+    float acc[8], m[8], l[8], most = big;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = s0 + i < a.splits;
+      const bool in = s0 + i < end;
       m[i] = in ? a.part_ml[(slot + s0 + i) * 2] : -INFINITY;
       l[i] = in ? a.part_ml[(slot + s0 + i) * 2 + 1] : 0.f;
       acc[i] = in ? a.part_acc[(slot + s0 + i) * D + dim] : 0.f;
     }
 #pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, m[i]);
+    const float f0 = big == most ? 1.f : fast_exp2(big - most);
+    num *= f0, den *= f0, big = most;
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - big);
       num = fmaf(f, acc[i], num);
       den = fmaf(f, l[i], den);      // (0 times a NaN is one: scores that are all none stay visible)
+    }
+  }
+  if constexpr (PARTS > 1) {
+    num_s[part][dim] = num;
+    if (dim == 0) m_s[part] = big, den_s[part] = den;
+    __syncthreads();
+    if (part > 0) return;
+    big = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) big = fmaxf(big, m_s[i]);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const float f = m_s[i] == -INFINITY ? 0.f : fast_exp2(m_s[i] - big);
+      num = fmaf(f, num_s[i][dim], num);
+      den = fmaf(f, den_s[i], den);
     }
   }
   a.out[(size_t)(qs + token) * a.out_stride + (size_t)head * D + dim] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
@@ -492,46 +557,74 @@ int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, dim3
   static LabShared granted;
   cudaError_t e = lab_allow_shared(granted, (const void*)attention_q8_few_kernel<N>, Layout<N>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  return (int)lab_launch(attention_q8_few_kernel<N>, grid, dim3(THREADS), (size_t)Layout<N>::SMEM, stream, mk, mv, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Layout<N>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (a.cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (g_lab_pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return (int)cudaLaunchKernelEx(&cfg, attention_q8_few_kernel<N>, mk, mv, a);
 }
 
 }  // namespace
 
-// Rows a CTA takes (the widths built), and floats of scratch that `splits` > 1 need.
-LAB_EXPORT long long lab_attention_q8_few_scratch(int tokens, int n_q, int splits) {
-  return splits > 1 ? (long long)tokens * n_q * splits * (D + 2) : 0;
-}
+// A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise; requests of up to most_rows rows (longer
+// ones are left alone), `longest` the most that one of them brings; width: rows a CTA takes, 16, 32 or 48; splits of the keys, merged
+// inside their cluster (`cluster`, up to eight) or by a second kernel through scratch: tokens * n_q * splits * (D + 2) floats.
+// window as lab_first_key takes it.
+struct LabQ8Few {
+  void* out;
+  const void *q, *k, *v, *k_scale, *v_scale;
+  const int *q_start, *kv_len, *pos0, *block_table;
+  float* scratch;
+  long long out_stride, q_stride;
+  int tokens, max_blocks, requests, n_q, n_kv, page_size, num_pages, window, most_rows, longest, width, splits, cluster;
+  float scale;
+};
 
-// Requests of up to most_rows rows (longer ones are left alone); `longest`: the most rows that one of them brings; width: rows a
-// CTA takes, 16, 32 or 48.  q and out as lab_attention_q8_any; scratch for splits > 1.
-LAB_EXPORT int lab_attention_q8_few(void* out, int out_stride, const void* q, long long q_stride, int tokens, const void* k, const void* v,
-                                    const void* k_scale, const void* v_scale, const int* q_start, const int* kv_len, const int* pos0,
-                                    const int* block_table, int max_blocks, int requests, int n_q, int n_kv, int page_size, int num_pages,
-                                    int window, float scale, int most_rows, int longest, int width, int splits, float* scratch,
-                                    cudaStream_t stream) {
-  if (tokens <= 0 || requests <= 0 || longest <= 0) return 0;
-  if (n_kv < 1 || n_q < 1 || n_q % n_kv || splits < 1 || max_blocks < 1 || longest > most_rows || (splits > 1 && scratch == nullptr) ||
-      !q8_pages_fit(page_size, (long long)num_pages * n_kv * page_size) || num_pages < 1 || q_stride % 2 ||
-      (((uintptr_t)q) & 3) || ((((uintptr_t)k) | ((uintptr_t)v)) & 15))
+LAB_EXPORT int lab_attention_q8_few(const LabQ8Few* c, cudaStream_t stream) {
+  if (c->tokens <= 0 || c->requests <= 0 || c->longest <= 0) return 0;
+  if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->splits < 1 || c->max_blocks < 1 || c->longest > c->most_rows ||
+      (c->cluster && (c->splits < 2 || c->splits > 8)) || (c->splits > 1 && !c->cluster && c->scratch == nullptr) ||
+      !q8_pages_fit(c->page_size, (long long)c->num_pages * c->n_kv * c->page_size) || c->num_pages < 1 || c->q_stride % 2 ||
+      c->requests > 65535 || c->n_q > 65535 || (((uintptr_t)c->q) & 3) || ((((uintptr_t)c->k) | ((uintptr_t)c->v)) & 15))
     return (int)cudaErrorInvalidValue;
   CUtensorMap mk, mv;
   int rc;
-  const long long rows = (long long)num_pages * n_kv * page_size;
-  if ((rc = q8_make_map<D>(&mk, k, rows, page_size))) return rc;
-  if ((rc = q8_make_map<D>(&mv, v, rows, page_size))) return rc;
+  const long long rows = (long long)c->num_pages * c->n_kv * c->page_size;
+  if ((rc = q8_make_map<D>(&mk, c->k, rows, c->page_size))) return rc;
+  if ((rc = q8_make_map<D>(&mv, c->v, rows, c->page_size))) return rc;
   Args a;
-  a.out = (__nv_bfloat16*)out, a.out_stride = out_stride, a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride;
-  a.k_scale = (const uint8_t*)k_scale, a.v_scale = (const uint8_t*)v_scale;
-  a.q_start = q_start, a.kv_len = kv_len, a.pos0 = pos0, a.block_table = block_table, a.max_blocks = max_blocks;
-  a.n_q = n_q, a.n_kv = n_kv, a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.most_rows = most_rows;
-  a.splits = splits, a.scale_log2 = scale * LOG2E;
-  a.part_acc = scratch, a.part_ml = scratch ? scratch + (size_t)tokens * n_q * splits * D : nullptr;
-  const int row_tiles = (longest * (n_q / n_kv) + width - 1) / width;
-  const dim3 grid(splits, n_kv * row_tiles, requests);
-  if (width == 16) rc = launch_few<16>(mk, mv, a, grid, stream);
-  else if (width == 32) rc = launch_few<32>(mk, mv, a, grid, stream);
-  else if (width == 48) rc = launch_few<48>(mk, mv, a, grid, stream);
+  a.out = (__nv_bfloat16*)c->out, a.out_stride = c->out_stride, a.q = (const __nv_bfloat16*)c->q, a.q_stride = c->q_stride;
+  a.k_scale = (const uint8_t*)c->k_scale, a.v_scale = (const uint8_t*)c->v_scale;
+  a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
+  a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window;
+  a.most_rows = c->most_rows, a.splits = c->splits, a.cluster = c->cluster, a.scale_log2 = c->scale * LOG2E;
+  const bool second = c->splits > 1 && !c->cluster;
+  a.part_acc = c->scratch, a.part_ml = second ? c->scratch + (size_t)c->tokens * c->n_q * c->splits * D : nullptr;
+  const int row_tiles = (c->longest * (c->n_q / c->n_kv) + c->width - 1) / c->width;
+  if ((long long)c->n_kv * row_tiles > 65535) return (int)cudaErrorInvalidValue;
+  const dim3 grid(c->splits, c->n_kv * row_tiles, c->requests);
+  if (c->width == 16) rc = launch_few<16>(mk, mv, a, grid, stream);
+  else if (c->width == 32) rc = launch_few<32>(mk, mv, a, grid, stream);
+  else if (c->width == 48) rc = launch_few<48>(mk, mv, a, grid, stream);
   else rc = (int)cudaErrorInvalidValue;
-  if (rc || splits == 1) return rc;
-  return (int)lab_launch(attention_q8_merge_kernel, dim3(longest, n_q, requests), dim3(D), 0, stream, a);
+  if (rc || !second) return rc;
+  const dim3 heads(c->longest, c->n_q, c->requests);
+  if (c->splits > 16) return (int)lab_launch(attention_q8_merge_kernel<MERGE_PARTS>, heads, dim3(MERGE_PARTS * D), 0, stream, a);
+  return (int)lab_launch(attention_q8_merge_kernel<1>, heads, dim3(D), 0, stream, a);
 }

@@ -431,28 +431,34 @@ LAB_EXPORT long long lab_attention_q8_rows_scratch(int many, int n_kv, int windo
   return (long long)many * n_kv * span_of(window, most_keys, longest) * D * 4;
 }
 
-// Requests of `fewest` rows or more (shorter ones are left alone), `many` of them; `longest`: the most rows that one of them
-// brings; lengths are at most most_keys.  q and out as lab_attention_q8_any, q's rows on 16-byte boundaries; scratch on a
-// boundary of 16 bytes.
-LAB_EXPORT int lab_attention_q8_rows(void* out, int out_stride, const void* q, long long q_stride, const void* k, const void* v,
-                                     const void* k_scale, const void* v_scale, const int* q_start, const int* kv_len, const int* pos0,
-                                     const int* block_table, int max_blocks, int requests, int n_q, int n_kv, int page_size, int num_pages,
-                                     int window, float scale, int fewest, int longest, int many, int most_keys, void* scratch,
-                                     cudaStream_t stream) {
-  if (requests <= 0 || longest <= 0 || many <= 0) return 0;
-  const int span = span_of(window, most_keys, longest);
-  const long long rows = (long long)many * n_kv * span;
-  if (n_kv < 1 || n_q < 1 || n_q % n_kv || max_blocks < 1 || num_pages < 1 || fewest < 1 || page_size < 1 || most_keys < 1 || rows >= (1ll << 31) ||
-      requests > 65535 || n_kv > 65535 || q_stride % 8 || (((uintptr_t)q) & 15) || ((((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)scratch)) & 15) ||
-      scratch == nullptr)
+// A call, as the host packs it.  q: rows q_stride elements apart, on 16-byte boundaries, out likewise; requests of `fewest` rows or
+// more (shorter ones are left alone), `many` of them, `longest` the most rows that one brings; lengths are at most most_keys;
+// scratch on a boundary of 16 bytes.  window as lab_first_key takes it.
+struct LabQ8Rows {
+  void* out;
+  const void *q, *k, *v, *k_scale, *v_scale;
+  const int *q_start, *kv_len, *pos0, *block_table;
+  void* scratch;
+  long long out_stride, q_stride;
+  int max_blocks, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys;
+  float scale;
+};
+
+LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
+  if (c->requests <= 0 || c->longest <= 0 || c->many <= 0) return 0;
+  const int span = span_of(c->window, c->most_keys, c->longest);
+  const long long rows = (long long)c->many * c->n_kv * span;
+  if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->max_blocks < 1 || c->num_pages < 1 || c->fewest < 1 || c->page_size < 1 ||
+      c->most_keys < 1 || rows >= (1ll << 31) || c->requests > 65535 || c->n_kv > 65535 || c->q_stride % 8 || (((uintptr_t)c->q) & 15) ||
+      ((((uintptr_t)c->k) | ((uintptr_t)c->v) | ((uintptr_t)c->scratch)) & 15) || c->scratch == nullptr)
     return (int)cudaErrorInvalidValue;
   Args a;
-  a.out = (__nv_bfloat16*)out, a.out_stride = out_stride, a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride;
-  a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.k_scale = (const uint8_t*)k_scale, a.v_scale = (const uint8_t*)v_scale;
-  a.q_start = q_start, a.kv_len = kv_len, a.pos0 = pos0, a.block_table = block_table, a.max_blocks = max_blocks;
-  a.n_q = n_q, a.n_kv = n_kv, a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.fewest = fewest, a.many = many;
-  a.wide_k = (__nv_bfloat16*)scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
-  a.scale_log2 = scale * LOG2E;
+  a.out = (__nv_bfloat16*)c->out, a.out_stride = c->out_stride, a.q = (const __nv_bfloat16*)c->q, a.q_stride = c->q_stride;
+  a.k = (const uint8_t*)c->k, a.v = (const uint8_t*)c->v, a.k_scale = (const uint8_t*)c->k_scale, a.v_scale = (const uint8_t*)c->v_scale;
+  a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
+  a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window, a.fewest = c->fewest;
+  a.many = c->many, a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
+  a.scale_log2 = c->scale * LOG2E;
   CUtensorMap mk, mv;
   int rc;
   if ((rc = lab_make_map_bf16(&mk, a.wide_k, rows, D, D, KEYS))) return rc;
@@ -460,9 +466,9 @@ LAB_EXPORT int lab_attention_q8_rows(void* out, int out_stride, const void* q, l
   static LabShared granted;
   cudaError_t e = lab_allow_shared(granted, (const void*)attention_q8_rows_kernel, SMEM);
   if (e != cudaSuccess) return (int)e;
-  e = lab_launch(widen_kernel, dim3(span / KEYS, n_kv, requests), dim3(WIDEN_THREADS), 0, stream, a);
-  if (e != cudaSuccess) return (int)e;
-  const long long tiles = ((long long)longest * (n_q / n_kv) + ROWS - 1) / ROWS;
+  const long long tiles = ((long long)c->longest * (c->n_q / c->n_kv) + ROWS - 1) / ROWS;
   if (tiles > 65535) return (int)cudaErrorInvalidValue;
-  return (int)lab_launch(attention_q8_rows_kernel, dim3(n_kv, (unsigned)tiles, requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
+  e = lab_launch(widen_kernel, dim3(span / KEYS, c->n_kv, c->requests), dim3(WIDEN_THREADS), 0, stream, a);
+  if (e != cudaSuccess) return (int)e;
+  return (int)lab_launch(attention_q8_rows_kernel, dim3(c->n_kv, (unsigned)tiles, c->requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
 }

@@ -339,38 +339,52 @@ int launch_load(T* out_k, T* out_v, const uint8_t* k, const uint8_t* v, const ui
 
 LAB_EXPORT int lab_q8_most_dim() { return MOST_DIM; }
 
-// rows: [tokens, row_stride] of `dtype`, or (parts > 0) [parts, tokens, width] floats whose sum with `bias` is rounded to
-// bfloat16 first; width = (n_q + 2 n_kv) d.  table: [tokens, rotary_dim / 2] (cos, sin).  q_out: [tokens, n_q * d].  Slots that
-// are not negative differ from one another.
-LAB_EXPORT int lab_rope_kv_store_q8(const void* rows, long long row_stride, int parts, long long part_stride, const void* bias,
-                                    const void* table, int rotary_dim, const int* slots, void* q_out, void* k, void* v, void* k_scale,
-                                    void* v_scale, int tokens, int n_q, int n_kv, int d, int page_size, int num_pages, int dtype,
-                                    cudaStream_t stream) {
-  if (tokens <= 0) return 0;
-  if (d < 1 || d > MOST_DIM || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > d || n_q < 0 || n_kv < 1 || page_size < 1 || num_pages < 0 ||
-      (long long)tokens * (n_q + 2 * n_kv) * 32 >= (1ll << 31) || parts < 0 || (parts > 0 && dtype != LAB_BF16) || (rotary_dim > 0 && table == nullptr))
+// A call, as the host packs it.  rows: [tokens, row_stride] of `dtype`, or (parts > 0) [parts, tokens, width] floats whose sum with
+// `bias` is rounded to bfloat16 first; width = (n_q + 2 n_kv) d.  table: [tokens, rotary_dim / 2] (cos, sin).  q_out: [tokens, n_q *
+// d].  Slots that are not negative differ from one another.
+struct LabQ8Store {
+  const void *rows, *bias, *table;
+  const int* slots;
+  void *q_out, *k, *v, *k_scale, *v_scale;
+  long long row_stride, part_stride;
+  int parts, rotary_dim, tokens, n_q, n_kv, d, page_size, num_pages, dtype;
+};
+
+LAB_EXPORT int lab_rope_kv_store_q8(const LabQ8Store* c, cudaStream_t stream) {
+  if (c->tokens <= 0) return 0;
+  const int parts = c->parts, d = c->d, rotary_dim = c->rotary_dim;
+  if (d < 1 || d > MOST_DIM || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > d || c->n_q < 0 || c->n_kv < 1 || c->page_size < 1 ||
+      c->num_pages < 0 || (long long)c->tokens * (c->n_q + 2 * c->n_kv) * 32 >= (1ll << 31) || parts < 0 ||
+      (parts > 0 && c->dtype != LAB_BF16) || (rotary_dim > 0 && c->table == nullptr))
     return (int)cudaErrorInvalidValue;
   Store s;
-  s.rows = rows, s.row_stride = row_stride, s.parts = parts, s.part_stride = part_stride, s.bias = (const __nv_bfloat16*)bias;
-  s.table = (const float2*)table, s.rotary_dim = rotary_dim, s.slots = slots, s.q_out = q_out;
-  s.k = (uint8_t*)k, s.v = (uint8_t*)v, s.k_scale = (uint8_t*)k_scale, s.v_scale = (uint8_t*)v_scale;
-  s.tokens = tokens, s.n_q = n_q, s.n_kv = n_kv, s.d = d, s.page_size = page_size, s.num_pages = num_pages;
-  const int size = parts > 0 || dtype == LAB_F32 ? 4 : 2;
-  const bool vec = rotary_dim == d && d >= 16 && d <= (parts > 0 ? 128 : 256) && (d & (d - 1)) == 0 && row_stride * size % 16 == 0 &&
-                   (parts == 0 || part_stride * size % 16 == 0) &&
-                   (((uintptr_t)rows | (uintptr_t)table | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
-  if (dtype == LAB_F32) return launch_store<float, false>(s, vec, stream);
+  s.rows = c->rows, s.row_stride = c->row_stride, s.parts = parts, s.part_stride = c->part_stride, s.bias = (const __nv_bfloat16*)c->bias;
+  s.table = (const float2*)c->table, s.rotary_dim = rotary_dim, s.slots = c->slots, s.q_out = c->q_out;
+  s.k = (uint8_t*)c->k, s.v = (uint8_t*)c->v, s.k_scale = (uint8_t*)c->k_scale, s.v_scale = (uint8_t*)c->v_scale;
+  s.tokens = c->tokens, s.n_q = c->n_q, s.n_kv = c->n_kv, s.d = d, s.page_size = c->page_size, s.num_pages = c->num_pages;
+  const int size = parts > 0 || c->dtype == LAB_F32 ? 4 : 2;
+  const bool vec = rotary_dim == d && d >= 16 && d <= (parts > 0 ? 128 : 256) && (d & (d - 1)) == 0 && c->row_stride * size % 16 == 0 &&
+                   (parts == 0 || c->part_stride * size % 16 == 0) &&
+                   (((uintptr_t)c->rows | (uintptr_t)c->table | (uintptr_t)c->q_out | (uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0;
+  if (c->dtype == LAB_F32) return launch_store<float, false>(s, vec, stream);
   return parts > 0 ? launch_store<__nv_bfloat16, true>(s, vec, stream) : launch_store<__nv_bfloat16, false>(s, vec, stream);
 }
 
 // out_k, out_v: [rows, n_kv, d] of `dtype`; a negative slot gives a row of zeros.
-LAB_EXPORT int lab_kv_load_q8(void* out_k, void* out_v, const void* k, const void* v, const void* k_scale, const void* v_scale,
-                              const int* slots, long long rows, int n_kv, int d, int page_size, int num_pages, int dtype,
-                              cudaStream_t stream) {
-  if (rows <= 0) return 0;
-  if (d < 1 || n_kv < 1 || page_size < 1 || num_pages < 0) return (int)cudaErrorInvalidValue;
-  const uint8_t *kc = (const uint8_t*)k, *vc = (const uint8_t*)v, *ks = (const uint8_t*)k_scale, *vs = (const uint8_t*)v_scale;
-  if (dtype == LAB_F32)
-    return launch_load((float*)out_k, (float*)out_v, kc, vc, ks, vs, slots, rows, n_kv, d, page_size, num_pages, stream);
-  return launch_load((__nv_bfloat16*)out_k, (__nv_bfloat16*)out_v, kc, vc, ks, vs, slots, rows, n_kv, d, page_size, num_pages, stream);
+struct LabQ8Load {
+  void *out_k, *out_v;
+  const void *k, *v, *k_scale, *v_scale;
+  const int* slots;
+  long long rows;
+  int n_kv, d, page_size, num_pages, dtype;
+};
+
+LAB_EXPORT int lab_kv_load_q8(const LabQ8Load* c, cudaStream_t stream) {
+  if (c->rows <= 0) return 0;
+  if (c->d < 1 || c->n_kv < 1 || c->page_size < 1 || c->num_pages < 0) return (int)cudaErrorInvalidValue;
+  const uint8_t *k = (const uint8_t*)c->k, *v = (const uint8_t*)c->v, *ks = (const uint8_t*)c->k_scale, *vs = (const uint8_t*)c->v_scale;
+  if (c->dtype == LAB_F32)
+    return launch_load((float*)c->out_k, (float*)c->out_v, k, v, ks, vs, c->slots, c->rows, c->n_kv, c->d, c->page_size, c->num_pages, stream);
+  return launch_load((__nv_bfloat16*)c->out_k, (__nv_bfloat16*)c->out_v, k, v, ks, vs, c->slots, c->rows, c->n_kv, c->d, c->page_size,
+                     c->num_pages, stream);
 }

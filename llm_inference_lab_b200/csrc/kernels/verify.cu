@@ -300,24 +300,38 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a,
 
 }  // namespace
 
-// Bytes of scratch a call needs.
-LAB_EXPORT long long lab_verify_scratch(int rows, int vocab) { return (long long)rows * ((vocab + CHUNK - 1) / CHUNK) * 16; }
+// A call needs 16 bytes of scratch a row and chunk of this many entries.
+LAB_EXPORT int lab_verify_chunk() { return CHUNK; }
 
-// logits [rows, vocab] 32-bit, rows `ld` apart; draft_probs likewise or null; drafts [rows]: the token drafted after a row's (a
-// request's last row has none); starts [requests + 1]; temperature, seeds, positions [requests], null: greedy.  tokens [rows]:
-// what a request's rows give, drafts that were accepted, the token that ends it, -1 behind it; counts [requests].
-LAB_EXPORT int lab_verify_drafts(int* tokens, int* counts, const float* logits, long long ld, const float* draft_probs, long long ld_probs,
-                                 const int* drafts, const int* starts, const float* temperature, const uint32_t* seeds,
-                                 const int* positions, int rows, int vocab, int requests, void* scratch, cudaStream_t stream) {
+// A call, as the host packs it.  logits [rows, vocab] 32-bit, rows `ld` apart; draft_probs likewise or null; drafts [rows]: the token
+// drafted after a row's (a request's last row has none); starts [requests + 1]; temperature, seeds, positions [requests], null:
+// greedy.  tokens [rows]: what a request's rows give, drafts that were accepted, the token that ends it, -1 behind it; counts
+// [requests].
+struct LabVerify {
+  int *tokens, *counts;
+  const float *logits, *draft_probs;
+  const int *drafts, *starts;
+  const float* temperature;
+  const uint32_t* seeds;
+  const int* positions;
+  void* scratch;
+  long long ld, ld_probs;
+  int rows, vocab, requests;
+};
+
+LAB_EXPORT int lab_verify_drafts(const LabVerify* c, cudaStream_t stream) {
+  const int rows = c->rows, vocab = c->vocab, requests = c->requests;
+  void* scratch = c->scratch;
+  const float* temperature = c->temperature;
   if (requests <= 0) return 0;
   if (rows < 0 || rows > 65535 || vocab < 1 || (rows > 0 && scratch == nullptr) || (((uintptr_t)scratch) & 15) ||
-      (temperature != nullptr && (seeds == nullptr || positions == nullptr)))
+      (temperature != nullptr && (c->seeds == nullptr || c->positions == nullptr)))
     return (int)cudaErrorInvalidValue;
   Args a;
-  a.logits = logits, a.ld = ld, a.draft_probs = draft_probs, a.ld_probs = ld_probs, a.drafts = drafts, a.starts = starts;
-  a.temperature = temperature, a.seeds = seeds, a.positions = positions;
+  a.logits = c->logits, a.ld = c->ld, a.draft_probs = c->draft_probs, a.ld_probs = c->ld_probs, a.drafts = c->drafts, a.starts = c->starts;
+  a.temperature = temperature, a.seeds = c->seeds, a.positions = c->positions;
   a.rows = rows, a.vocab = vocab, a.requests = requests, a.chunks = (vocab + CHUNK - 1) / CHUNK;
-  a.part = (float4*)scratch, a.tokens = tokens, a.counts = counts;
+  a.part = (float4*)scratch, a.tokens = c->tokens, a.counts = c->counts;
   if (rows > 0) {
     const cudaError_t e = lab_launch(verify_chunks_kernel, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
     if (e != cudaSuccess) return (int)e;

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 import threading
 from typing import NamedTuple
 
@@ -2354,31 +2355,73 @@ def quant_pages(num_pages: int, n_kv: int, page_size: int, head_dim: int, device
     return QuantPages(code(), code(), byte(), byte())
 
 
+# The calls of these operators hand one packed record to the library (a struct of the .cu file, members in its order): two dozen
+# arguments one by one cost the host 9 microseconds, a record 3.5.  Likewise an operator looks at its arguments in one expression,
+# and only where that does not hold goes through them again to say which it is.
+_E4M3, _BYTE, _INT = torch.float8_e4m3fn, torch.uint8, torch.int32
+_device_now = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_pack_store = struct.Struct("9P2q9i").pack
+_pack_load = struct.Struct("7Pq5i").pack
+_pack_any = struct.Struct("10P2q10if").pack
+_pack_few = struct.Struct("11P2q13if").pack
+_pack_rows = struct.Struct("11P2q11if").pack
+_pack_verify = struct.Struct("10P2q3i").pack
+
+
+_entries: dict = {}    # (library, entry, head size) -> the entry, which takes a record and a stream
+
+
+def _entry(library: str, entry: str, head_dim: int = 0):
+    f = _entries.get((library, entry, head_dim))
+    if f is None:
+        f = lib(library, {"LAB_HEAD_DIM": head_dim} if head_dim else None)[entry]
+        f.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        _entries[library, entry, head_dim] = f
+    return f
+
+
+def _current(device: int) -> int:
+    """The current stream of the current device (which `device` is)."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
 def _require(ok: bool, what: str) -> None:
     if not ok:
         raise KernelError(what)
 
 
-def _same_device(what: str, first: torch.Tensor, *tensors) -> None:
-    """All on the device of `first`, which is the current one: the kernel is launched on the current stream."""
+def _place(what: str, first: torch.Tensor, *tensors) -> None:
+    """Raises unless all are on one GPU, the current device: the kernel is launched on the current stream."""
     _on_gpu(first, *tensors)
     _require(all(t is None or t.device == first.device for t in tensors), f"{what}: tensors on different devices")
     _require(first.device.index == torch.cuda.current_device(),
              f"{what}: tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    raise KernelError(f"{what}: arguments refused")
 
 
-def _q8_pages(what: str, pages: QuantPages, n_kv: int, head_dim: int) -> tuple[int, int]:
-    """Checks a cache's pages; (pages, page size)."""
+def _pages_fit(pages: QuantPages, device: int, n_kv: int, head_dim: int) -> bool:
+    k, v, ks, vs = pages
+    shape, rows = k.shape, ks.shape
+    return (len(shape) == 4 and shape[1] == n_kv and shape[3] == head_dim and v.shape == shape and rows == shape[:3] and vs.shape == rows
+            and k.dtype is _E4M3 and v.dtype is _E4M3 and ks.dtype is _BYTE and vs.dtype is _BYTE and k.is_contiguous() and v.is_contiguous()
+            and ks.is_contiguous() and vs.is_contiguous() and k.get_device() == device and v.get_device() == device
+            and ks.get_device() == device and vs.get_device() == device)
+
+
+def _refuse_pages(what: str, pages: QuantPages, n_kv: int, head_dim: int) -> None:
     _require(pages.k.dim() == 4 and tuple(pages.k.shape[1::2]) == (n_kv, head_dim),
              f"{what}: pages of shape {tuple(pages.k.shape)} are not [pages, {n_kv}, page_size, {head_dim}]")
-    for t, dtype, shape in ((pages.k, torch.float8_e4m3fn, pages.k.shape), (pages.v, torch.float8_e4m3fn, pages.k.shape),
-                            (pages.k_scale, torch.uint8, pages.k.shape[:3]), (pages.v_scale, torch.uint8, pages.k.shape[:3])):
+    for t, dtype, shape in ((pages.k, _E4M3, pages.k.shape), (pages.v, _E4M3, pages.k.shape),
+                            (pages.k_scale, _BYTE, pages.k.shape[:3]), (pages.v_scale, _BYTE, pages.k.shape[:3])):
         _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
                  f"{what}: pages hold contiguous float8_e4m3fn codes and uint8 scales of one shape, got {t.dtype} {tuple(t.shape)}")
-    return pages.k.shape[0], pages.k.shape[2]
 
 
-def _integers(what: str, name: str, t: torch.Tensor, count: int) -> None:
+def _ints_fit(t: torch.Tensor, device: int, count: int) -> bool:
+    return t.dtype is _INT and t.is_contiguous() and t.numel() >= count and t.get_device() == device
+
+
+def _refuse_ints(what: str, name: str, t: torch.Tensor, count: int) -> None:
     _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= count,
              f"{what}: {name} holds {count} int32 numbers or more, contiguous, got {t.dtype} {tuple(t.shape)}")
 
@@ -2392,49 +2435,72 @@ def rope_kv_store_q8(qkv: torch.Tensor, table: torch.Tensor | None, rotary_dim: 
     tokens, ..] whose sum with `bias` is rounded to bfloat16 first (contiguous); `table` comes from `rope_table` (None with
     rotary_dim 0).  Slots that are not negative differ from one another.  A code is what the exact rotated number rounds to, in
     one rounding; a row with a number that is not finite reads back as NaN.  Head sizes up to 256."""
+    shape, device, kind = qkv.shape, qkv.get_device(), qkv.dtype
+    parts = shape[0] if len(shape) == 3 else 0
+    tokens, width = shape[-2] if len(shape) > 1 else 0, (n_q + 2 * n_kv) * head_dim
+    k, v, ks, vs = pages
+    if not (2 <= len(shape) <= 3 and shape[-1] == width and 0 <= rotary_dim <= head_dim <= 256 and rotary_dim % 2 == 0 and device >= 0
+            and device == _device_now() and _ints_fit(slots, device, tokens) and _pages_fit(pages, device, n_kv, head_dim)
+            and (qkv.is_contiguous() and kind is torch.float32 if parts else len(shape) == 2 and qkv.stride(1) == 1 and
+                 (kind is torch.bfloat16 or kind is torch.float32))
+            and (bias is None or (parts and bias.dtype is torch.bfloat16 and bias.is_contiguous() and bias.numel() == width
+                                  and bias.get_device() == device))
+            and (rotary_dim == 0 or (table is not None and table.dtype is torch.float32 and table.is_contiguous()
+                                     and table.shape == (tokens, rotary_dim // 2, 2) and table.get_device() == device))):
+        _refuse_store(qkv, table, rotary_dim, slots, pages, n_q, n_kv, head_dim, bias)
+    bf16 = parts or kind is torch.bfloat16
+    q = torch.empty((tokens, n_q * head_dim), dtype=torch.bfloat16 if bf16 else kind, device=qkv.device)
+    _check(_entry("quant_cache", "lab_rope_kv_store_q8")(_pack_store(
+        qkv.data_ptr(), bias.data_ptr() if bias is not None else 0, table.data_ptr() if rotary_dim else 0, slots.data_ptr(), q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), qkv.stride(-2), tokens * width, parts, rotary_dim, tokens, n_q, n_kv, head_dim,
+        k.shape[2], k.shape[0], BF16 if bf16 else F32), _current(device)), "rope_kv_store_q8")
+    return q
+
+
+def _refuse_store(qkv, table, rotary_dim, slots, pages, n_q, n_kv, head_dim, bias):
     what = "rope_kv_store_q8"
-    parts = qkv.shape[0] if qkv.dim() == 3 else 0
     _require(qkv.dim() in (2, 3), f"{what}: rows or partial products, got {tuple(qkv.shape)}")
-    tokens, width = qkv.shape[-2], (n_q + 2 * n_kv) * head_dim
-    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
-    _require( qkv.shape[-1] == width and qkv.stride(-1) == 1,
+    parts, (tokens, width) = qkv.shape[0] if qkv.dim() == 3 else 0, (qkv.shape[-2], (n_q + 2 * n_kv) * head_dim)
+    _refuse_pages(what, pages, n_kv, head_dim)
+    _require(qkv.shape[-1] == width and qkv.stride(-1) == 1,
              f"{what}: rows of {width} = (n_q + 2 n_kv) * head_dim neighbouring numbers, got {tuple(qkv.shape)}")
-    _require(parts == 0 or (qkv.dtype == torch.float32 and qkv.is_contiguous()), f"{what}: partial products are contiguous float32")
+    _require(qkv.dim() == 2 or (parts > 0 and qkv.dtype == torch.float32 and qkv.is_contiguous()), f"{what}: partial products are contiguous float32")
     _require(bias is None or (parts > 0 and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == width),
              f"{what}: a bias of {width} bfloat16 numbers goes with partial products")
     _require(0 <= rotary_dim <= head_dim <= 256 and rotary_dim % 2 == 0, f"{what}: head size {head_dim} up to 256, rotary_dim {rotary_dim} even")
     _require(rotary_dim == 0 or (table is not None and table.dtype == torch.float32 and table.is_contiguous()
                                  and tuple(table.shape) == (tokens, rotary_dim // 2, 2)),
              f"{what}: a table [{tokens}, {rotary_dim // 2}, 2] of cosines and sines, float32 and contiguous")
-    _integers(what, "slots", slots, tokens)
-    dt = torch.bfloat16 if parts else qkv.dtype
-    code = dtype_code(dt)
-    _same_device(what, qkv, table, slots, bias, *pages)
-    q = torch.empty((tokens, n_q * head_dim), dtype=dt, device=qkv.device)
-    _check(lib("quant_cache").lab_rope_kv_store_q8(
-        _ptr(qkv), ctypes.c_longlong(qkv.stride(-2)), parts, ctypes.c_longlong(tokens * width), _ptr(bias), _ptr(table if rotary_dim else None),
-        rotary_dim, _ptr(slots), _ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), tokens, n_q, n_kv,
-        head_dim, page_size, num_pages, code, _stream()), what)
-    return q
+    _refuse_ints(what, "slots", slots, tokens)
+    dtype_code(qkv.dtype)
+    _place(what, qkv, table, slots, bias, *pages)
 
 
 def kv_load_q8(pages: QuantPages, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values at `slots` of an 8-bit cache as numbers: k, v [rows, n_kv, head_dim] of `dtype` (both types hold them
     exactly).  A negative slot gives a row of zeros; a slot may come more than once."""
+    codes, v_codes, ks, vs = pages
+    shape, device = codes.shape, slots.get_device()
+    if not (len(shape) == 4 and slots.dim() == 1 and device >= 0 and device == _device_now() and _ints_fit(slots, device, 0)
+            and _pages_fit(pages, device, shape[1], shape[3]) and (dtype is torch.bfloat16 or dtype is torch.float32)):
+        _refuse_load(pages, slots, dtype)
+    num_pages, n_kv, page_size, head_dim = shape
+    rows = slots.numel()
+    k, v = torch.empty((2, rows, n_kv, head_dim), dtype=dtype, device=slots.device).unbind(0)
+    _check(_entry("quant_cache", "lab_kv_load_q8")(_pack_load(
+        k.data_ptr(), v.data_ptr(), codes.data_ptr(), v_codes.data_ptr(), ks.data_ptr(), vs.data_ptr(), slots.data_ptr(), rows, n_kv, head_dim,
+        page_size, num_pages, BF16 if dtype is torch.bfloat16 else F32), _current(device)), "kv_load_q8")
+    return k, v
+
+
+def _refuse_load(pages, slots, dtype):
     what = "kv_load_q8"
     _require(pages.k.dim() == 4, f"{what}: pages of shape {tuple(pages.k.shape)} are not [pages, n_kv, page_size, head_dim]")
-    n_kv, head_dim = pages.k.shape[1], pages.k.shape[3]
-    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
+    _refuse_pages(what, pages, pages.k.shape[1], pages.k.shape[3])
     _require(slots.dim() == 1, f"{what}: one row of slots")
-    _integers(what, "slots", slots, slots.numel())
-    rows, code = slots.numel(), dtype_code(dtype)
-    _same_device(what, slots, *pages)
-    k = torch.empty((rows, n_kv, head_dim), dtype=dtype, device=slots.device)
-    v = torch.empty_like(k)
-    _check(lib("quant_cache").lab_kv_load_q8(
-        _ptr(k), _ptr(v), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(slots), ctypes.c_longlong(rows),
-        n_kv, head_dim, page_size, num_pages, code, _stream()), what)
-    return k, v
+    _refuse_ints(what, "slots", slots, slots.numel())
+    dtype_code(dtype)
+    _place(what, slots, *pages)
 
 
 # Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, which splits the keys.
@@ -2461,62 +2527,82 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     counts.  A row that sees no key is 0; rows of no request stay as they are.
 
     bfloat16 queries of heads of 64 and 128 over pages of 8 to 128 (a power of two) run on the tensor cores; 32-bit queries (in
-    32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units."""
+    32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `Q8_FEW_ROWS` rows
+    and query heads of a kv head take scratch for their keys and values in bfloat16, as many as their rows see."""
+    k, v, ks, vs = pages
+    device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
+    if not (q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1 and (kind is torch.bfloat16 or kind is torch.float32)
+            and n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256 and scale > 0 and len(q_lens) == n_requests
+            and len(table_shape) == 2 and table_shape[0] >= n_requests and device >= 0 and device == _device_now()
+            and _pages_fit(pages, device, n_kv, head_dim) and _ints_fit(q_start, device, n_requests + 1) and _ints_fit(kv_len, device, n_requests)
+            and _ints_fit(pos0, device, n_requests) and _ints_fit(block_table, device, 0)
+            and (out is None or (out.dtype is kind and out.shape == q.shape and out.stride(1) == 1 and out.get_device() == device))):
+        _refuse_attention(q, pages, q_start, kv_len, pos0, block_table, n_requests, q_lens, n_q, n_kv, head_dim, scale, out)
+    if out is None:
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=kind, device=q.device)
+    tokens, longest, stride = q.shape[0], max(q_lens, default=0), q.stride(0)
+    if longest == 0 or tokens == 0:
+        return out
+    num_pages, page_size, blocks, group = k.shape[0], k.shape[2], table_shape[1], n_q // n_kv
+    at, stream = q.data_ptr(), _current(device)
+    tensors = (out.data_ptr(), at, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+               pos0.data_ptr(), block_table.data_ptr())
+    if not (kind is torch.bfloat16 and (head_dim == 64 or head_dim == 128) and page_size in (8, 16, 32, 64, 128) and stride % 2 == 0 and at % 4 == 0
+            and blocks > 0 and num_pages > 0 and not _force_plain):
+        _check(_entry("attention_q8", "lab_attention_q8_any")(_pack_any(
+            *tensors, out.stride(0), stride, tokens, blocks, n_requests, n_q, n_kv, head_dim, page_size, num_pages, window,
+            BF16 if kind is torch.bfloat16 else F32, scale), stream), "attention_q8")
+        return out
+    # requests of up to `few` rows, and those of more
+    few = max(1, Q8_FEW_ROWS // group) if stride % 8 == 0 and at % 16 == 0 else longest
+    longest_few = longest
+    if longest > few:
+        longest_few = max((n for n in q_lens if n <= few), default=0)
+        L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
+        L.lab_attention_q8_rows_scratch.restype = ctypes.c_longlong
+        many = sum(1 for n in q_lens if n > few)
+        scratch = torch.empty((int(L.lab_attention_q8_rows_scratch(many, n_kv, window, max_kv_len, longest)),), dtype=_BYTE, device=q.device)
+        _check(_entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)(_pack_rows(
+            *tensors, scratch.data_ptr(), out.stride(0), stride, blocks, n_requests, n_q, n_kv, page_size, num_pages, window, few + 1, longest,
+            many, max_kv_len, scale), stream), "attention_q8", 2)
+    if longest_few:
+        wide = q8_few_width(longest_few * group)
+        if longest_few == 1 and longest == 1:
+            ctas = n_kv * -(-group // wide) * sum(q_lens)
+        else:
+            ctas = n_kv * sum(-(-n * group // wide) for n in q_lens if n <= few)
+        splits = q8_few_splits(ctas, wide, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few))
+        cluster = 2 <= splits <= 8
+        scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 8 else None
+        _check(_entry("attention_q8_few", "lab_attention_q8_few", head_dim)(_pack_few(
+            *tensors, scratch.data_ptr() if scratch is not None else 0, out.stride(0), stride, tokens, blocks, n_requests, n_q, n_kv, page_size,
+            num_pages, window, few, longest_few, wide, splits, cluster, scale), stream), "attention_q8", 1 if scratch is None else 2)
+    return out
+
+
+def _refuse_attention(q, pages, q_start, kv_len, pos0, block_table, n_requests, q_lens, n_q, n_kv, head_dim, scale, out):
     what = "attention_q8"
-    num_pages, page_size = _q8_pages(what, pages, n_kv, head_dim)
-    tokens, width = q.shape[0], n_q * head_dim
+    _refuse_pages(what, pages, n_kv, head_dim)
+    width = n_q * head_dim
     _require(q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1, f"{what}: q of {width} neighbouring numbers a row, got {tuple(q.shape)}")
     _require(n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
     _require(scale > 0, f"{what}: the scale is positive")
     for name, t, count in (("q_start", q_start, n_requests + 1), ("kv_len", kv_len, n_requests), ("pos0", pos0, n_requests)):
-        _integers(what, name, t, count)
-    _integers(what, "block_table", block_table, 0)
+        _refuse_ints(what, name, t, count)
+    _refuse_ints(what, "block_table", block_table, 0)
     _require(block_table.dim() == 2 and block_table.shape[0] >= n_requests, f"{what}: a row of the block table per request")
     _require(len(q_lens) == n_requests, f"{what}: the host's row counts, one per request")
-    _require(out is None or (out.dtype == q.dtype and tuple(out.shape) == (tokens, width) and out.stride(1) == 1), f"{what}: out as q")
-    code = dtype_code(q.dtype)
-    _same_device(what, q, q_start, kv_len, pos0, block_table, out, *pages)
-    if out is None:
-        out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
-    if not q_lens or max(q_lens) == 0 or tokens == 0:
-        return out
-    if code == BF16 and not _force_plain and head_dim in (64, 128) and page_size in (8, 16, 32, 64, 128) and q.stride(0) % 2 == 0 \
-            and q.data_ptr() % 4 == 0 and block_table.shape[1] > 0 and num_pages > 0:
-        group = n_q // n_kv
-        # requests of up to `few` rows, and those of more
-        few = max(1, Q8_FEW_ROWS // group) if q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else max(q_lens)
-        longest, longest_few = max(q_lens), max((n for n in q_lens if n <= few), default=0)
-        if longest > few:
-            L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
-            L.lab_attention_q8_rows_scratch.restype = ctypes.c_longlong
-            many = sum(1 for n in q_lens if n > few)
-            scratch = torch.empty((int(L.lab_attention_q8_rows_scratch(many, n_kv, window, max_kv_len, longest)),), dtype=torch.uint8, device=q.device)
-            _check(L.lab_attention_q8_rows(
-                _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
-                _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q,
-                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few + 1, longest, many, max_kv_len, _ptr(scratch), _stream()),
-                what, 2)
-        if longest_few:
-            width = q8_few_width(longest_few * group)
-            ctas = sum(n_kv * -(-n * group // width) for n in q_lens if n <= few)
-            splits = q8_few_splits(ctas, width, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few))
-            scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
-            _check(lib("attention_q8_few", {"LAB_HEAD_DIM": head_dim}).lab_attention_q8_few(
-                _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
-                _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q,
-                n_kv, page_size, num_pages, window, ctypes.c_float(scale), few, longest_few, width, splits, _ptr(scratch), _stream()),
-                what, 2 if splits > 1 else 1)
-        return out
-    _check(lib("attention_q8").lab_attention_q8_any(
-        _ptr(out), out.stride(0), _ptr(q), ctypes.c_longlong(q.stride(0)), tokens, _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale),
-        _ptr(pages.v_scale), _ptr(q_start), _ptr(kv_len), _ptr(pos0), _ptr(block_table), block_table.shape[1], n_requests, n_q, n_kv,
-        head_dim, page_size, num_pages, window, ctypes.c_float(scale), code, _stream()), what)
-    return out
+    _require(out is None or (out.dtype == q.dtype and out.shape == q.shape and out.stride(1) == 1), f"{what}: out as q")
+    dtype_code(q.dtype)
+    _place(what, q, q_start, kv_len, pos0, block_table, out, *pages)
 
 
 # ----------------------------------------------------------------------------------------
 # Drafted tokens (csrc/kernels/verify.cu)
 # ----------------------------------------------------------------------------------------
+_verify_chunk = 0     # entries of a row that a block of the first kernel takes, as the library says
+
+
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tensor, draft_probs: torch.Tensor | None = None,
                   temperature: torch.Tensor | None = None, seeds: torch.Tensor | None = None, positions: torch.Tensor | None = None):
     """Judges drafted tokens by the target's 32-bit logits [rows, vocab] and draws the token that follows the accepted ones.
@@ -2529,12 +2615,41 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tens
 
     Returns (tokens [rows], counts [requests]), int32: counts[b] tokens from row starts[b] on, drafts that were accepted and then
     the drawn one, -1 behind them.  A row without any number gives INT32_MAX, as `sample` does."""
+    shape, device, requests = logits.shape, logits.get_device(), starts.numel() - 1
+    if not (len(shape) == 2 and logits.dtype is torch.float32 and logits.stride(1) == 1 and 0 < shape[1] and shape[0] <= 65535 and device >= 0
+            and device == _device_now() and _ints_fit(drafts, device, shape[0]) and _ints_fit(starts, device, 1)
+            and (draft_probs is None or (draft_probs.dtype is torch.float32 and draft_probs.shape == shape and draft_probs.stride(1) == 1
+                                         and draft_probs.get_device() == device))
+            and (temperature is None or (seeds is not None and positions is not None and temperature.dtype is torch.float32
+                                         and temperature.is_contiguous() and temperature.numel() >= requests
+                                         and temperature.get_device() == device and _ints_fit(seeds, device, requests)
+                                         and _ints_fit(positions, device, requests)))):
+        _refuse_verify(logits, drafts, starts, draft_probs, temperature, seeds, positions)
+    global _verify_chunk
+    if _verify_chunk == 0:
+        _verify_chunk = int(lib("verify").lab_verify_chunk())
+    rows, vocab = shape
+    # results and the rows' partial results (16 bytes a chunk, on their boundary) in one allocation
+    behind = 4 * rows * -(-vocab // _verify_chunk)
+    room = torch.empty((behind + rows + requests,), dtype=_INT, device=logits.device)
+    at = room.data_ptr()
+    tokens, counts = room[behind: behind + rows], room[behind + rows:]
+    drawn = temperature is not None
+    _check(_entry("verify", "lab_verify_drafts")(_pack_verify(
+        at + 4 * behind, at + 4 * (behind + rows), logits.data_ptr(), draft_probs.data_ptr() if draft_probs is not None else 0,
+        drafts.data_ptr(), starts.data_ptr(), temperature.data_ptr() if drawn else 0, seeds.data_ptr() if drawn else 0,
+        positions.data_ptr() if drawn else 0, at, logits.stride(0), draft_probs.stride(0) if draft_probs is not None else 0, rows, vocab,
+        requests), _current(device)), "verify_drafts", 2 if rows else 1)
+    return tokens, counts
+
+
+def _refuse_verify(logits, drafts, starts, draft_probs, temperature, seeds, positions):
     what = "verify_drafts"
     _require(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1 and logits.shape[1] > 0,
              f"{what}: logits are float32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
-    rows, vocab = logits.shape
-    _integers(what, "drafts", drafts, rows)
-    _integers(what, "starts", starts, 1)
+    rows = logits.shape[0]
+    _refuse_ints(what, "drafts", drafts, rows)
+    _refuse_ints(what, "starts", starts, 1)
     _require(rows <= 65535, f"{what}: up to 65535 rows, got {rows}")
     requests = starts.numel() - 1
     _require(draft_probs is None or (draft_probs.dtype == torch.float32 and draft_probs.shape == logits.shape and draft_probs.stride(1) == 1),
@@ -2543,17 +2658,6 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tens
         _require(temperature.dtype == torch.float32 and temperature.is_contiguous() and temperature.numel() >= requests,
                  f"{what}: a float32 temperature per request")
         _require(seeds is not None and positions is not None, f"{what}: a temperature needs seeds and positions")
-        _integers(what, "seeds", seeds, requests)
-        _integers(what, "positions", positions, requests)
-    _same_device(what, logits, drafts, starts, draft_probs, temperature, seeds, positions)
-    tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    counts = torch.empty((requests,), dtype=torch.int32, device=logits.device)
-    L = lib("verify")
-    L.lab_verify_scratch.restype = ctypes.c_longlong
-    scratch = torch.empty((max(1, int(L.lab_verify_scratch(rows, vocab))),), dtype=torch.uint8, device=logits.device)
-    _check(L.lab_verify_drafts(
-        _ptr(tokens), _ptr(counts), _ptr(logits), ctypes.c_longlong(logits.stride(0)), _ptr(draft_probs),
-        ctypes.c_longlong(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(drafts), _ptr(starts), _ptr(temperature),
-        _ptr(seeds if temperature is not None else None), _ptr(positions if temperature is not None else None), rows, vocab, requests,
-        _ptr(scratch), _stream()), what, 2 if rows else 1)
-    return tokens, counts
+        _refuse_ints(what, "seeds", seeds, requests)
+        _refuse_ints(what, "positions", positions, requests)
+    _place(what, logits, drafts, starts, draft_probs, temperature, seeds, positions)
