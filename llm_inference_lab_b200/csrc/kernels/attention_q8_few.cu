@@ -33,6 +33,7 @@ constexpr int KEYS = Tile::KEYS;
 constexpr int THREADS = 192;
 constexpr int STAGES = D == 64 ? 4 : 2;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FROM_CODES = 0.00390625f;      // p' is formed 2^8 times too large
 
 template <int N> struct Layout {
   static constexpr int OFF_Q = 0;                                 // high, then low codes: [N, D] swizzled as the keys
@@ -73,6 +74,12 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[2]) {
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
 
 template <int N>
@@ -121,6 +128,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     bar->abort_flag = 0;
     mbar_init_fence();
   }
+  if (warp == 0 && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &map_k : &map_v) : "memory");
   if (warp == 1) tmem_alloc(&bar->tmem_slot, L::TMEM);
   tc_fence_before();
   __syncthreads();
@@ -223,29 +231,38 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     float* base_w = reinterpret_cast<float*>(smem + L::OFF_WARP) + w * 4 * N;      // [N] base, [N] rescale, [2][N] share
     float *rescale_w = base_w + N, *share_w = base_w + 2 * N;
     // q: scaled by a power of two per row, in two codes
-    for (int n = w; n < N; n += 4) {
-      const int r = r0 + n, token = r / group, head = kvh * group + r - token * group;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      const int at = lane * (D / 32);
-      if (n < n_rows) {
-        const __nv_bfloat16* src = a.q + (size_t)(qs + token) * a.q_stride + (size_t)head * D + at;
+    constexpr int MINE = N / 4, EACH = D / 32;      // rows of a warp (w, w + 4, ..), numbers of a row a lane
+    uint32_t x[MINE][EACH / 2];
 #pragma unroll
-        for (int e = 0; e < D / 32; e += 2) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(src + e);
-          x[e] = __uint_as_float(v << 16), x[e + 1] = __uint_as_float(v & 0xffff0000u);
-        }
+    for (int i = 0; i < MINE; ++i) {      // all loads in flight together
+      const int n = w + 4 * i, r = r0 + n, token = r / group, head = kvh * group + r - token * group;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(a.q + (size_t)(qs + token) * a.q_stride + (size_t)head * D + lane * EACH);
+#pragma unroll
+      for (int e = 0; e < EACH / 2; ++e) x[i][e] = n < n_rows ? src[e] : 0u;
+      if (lane == 0) {
+        const int pos = p0 + token;
+        row_last[n] = n < n_rows ? min(pos, last) : -1;
+        row_first[n] = lab_first_key(pos, a.window);
       }
-      uint32_t top = 0;
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    for (int i = 0; i < MINE; ++i) {
+      const int n = w + 4 * i;
+      uint32_t top = 0;      // of the numbers' upper 16 bits
+#pragma unroll
+      for (int e = 0; e < EACH / 2; ++e) top = max(top, max(x[i][e] & 0x7fff0000u, (x[i][e] << 16) & 0x7fff0000u));
       top = __reduce_max_sync(0xffffffffu, top);
       const int byte = q8_byte(top);
-      const float inverse = byte == Q8_NAN_BYTE ? 0.f : q8_inverse(byte);
+      const float inverse = q8_inverse(min(byte, 253));
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (byte != Q8_NAN_BYTE) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = byte == Q8_NAN_BYTE ? 0.f : x[e] * inverse;
+        for (int e = 0; e < EACH / 2; ++e)
+          f[2 * e] = __uint_as_float(x[i][e] << 16) * inverse, f[2 * e + 1] = __uint_as_float(x[i][e] & 0xffff0000u) * inverse;
+      }
       uint32_t high, low;
-      q8_split4(x, high, low);
-      uint8_t* to = smem + L::OFF_Q + Tile::piece_at(n, at >> 4) + (at & 15);
+      q8_split4(f, high, low);
+      uint8_t* to = smem + L::OFF_Q + Tile::piece_at(n, lane * EACH >> 4) + (lane * EACH & 15);
       if constexpr (D == 128) {
         *reinterpret_cast<uint32_t*>(to) = high;
         *reinterpret_cast<uint32_t*>(to + N * D) = low;
@@ -253,12 +270,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
         *reinterpret_cast<uint16_t*>(to) = (uint16_t)high;
         *reinterpret_cast<uint16_t*>(to + N * D) = (uint16_t)low;
       }
-      if (lane == 0) {
-        const int pos = p0 + token;
-        factor[n] = n < n_rows ? a.scale_log2 * q8_scale(byte) : 0.f;
-        row_last[n] = n < n_rows ? min(pos, last) : -1;
-        row_first[n] = lab_first_key(pos, a.window);
-      }
+      if (lane == 0) factor[n] = n < n_rows ? a.scale_log2 * q8_scale(byte) : 0.f;
     }
     proxy_fence();
     asm volatile("bar.sync 2, 128;" ::: "memory");      // the rows' numbers
@@ -297,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
       const int key = (t_lo + j) * KEYS + mine, key0 = (t_lo + j) * KEYS;
       const bool held = row >= 0;
       const bool unit = held && vb == 127;
-      float vexp = (float)((int)vb - 127), v_inv = __uint_as_float((uint32_t)(254 - min(vb, 253u)) << 23) * 0.00390625f;
+      float vexp = (float)((int)vb - 127), v_inv = __uint_as_float((uint32_t)(254 - min(vb, 253u)) << 23) * FROM_CODES;
       const float ks = vb == Q8_NAN_BYTE ? q8_scale(Q8_NAN_BYTE) : q8_scale(kb);      // a value that is no number, as a score that is none
       if (j + 1 < n_tiles) {      // the next key's bytes arrive beside this tile
         row = row_of(key + KEYS);
@@ -312,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
           uint32_t any = 0;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) any |= z[c].x | z[c].y | z[c].z | z[c].w;
-          if ((any & 0x7f7f7f7fu) == 0) vexp = Q8_LEAST_POWER, v_inv = __uint_as_float((uint32_t)(127 - Q8_LEAST_POWER) << 23) * 0.00390625f;
+          if ((any & 0x7f7f7f7fu) == 0) vexp = Q8_LEAST_POWER, v_inv = __uint_as_float((uint32_t)(127 - Q8_LEAST_POWER) << 23) * FROM_CODES;
         }
       }
       const int sb = j & 1;
@@ -447,21 +459,24 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
       }
     }
     if (ok && (D == 128 || lane < 16)) {
+      if (a.cluster) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (n >= n_rows) continue;
-        const float4 s4 = load4(sums + n * 4);
-        const float sum = (s4.x + s4.y) + (s4.z + s4.w);
-        const int r = r0 + n, token = r / group, head = kvh * group + r - token * group;
-        const float num = acc[n] * 0.00390625f;
-        if (a.cluster) {
-          own[n * D + dim] = num;
-        } else if (a.splits == 1) {
-          a.out[(size_t)(qs + token) * a.out_stride + (size_t)head * D + dim] = __float2bfloat16_rn(sum == 0.f ? 0.f : num / sum);
-        } else {
-          const size_t slot = ((size_t)(qs + token) * a.n_q + head) * a.splits + split;
-          a.part_acc[slot * D + dim] = num;
-          if (dim == 0) a.part_ml[slot * 2] = base_w[n], a.part_ml[slot * 2 + 1] = sum;
+        for (int n = 0; n < N; ++n) own[n * D + dim] = acc[n];
+      } else {
+        int token = r0 / group, head = r0 - token * group;      // of the row, counted on
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n >= n_rows) break;
+          const float4 s4 = load4(sums + n * 4);
+          const float sum = (s4.x + s4.y) + (s4.z + s4.w), num = acc[n] * FROM_CODES;
+          if (a.splits == 1) {
+            a.out[(size_t)(qs + token) * a.out_stride + (size_t)(kvh * group + head) * D + dim] = __float2bfloat16_rn(sum == 0.f ? 0.f : num / sum);
+          } else {
+            const size_t slot = ((size_t)(qs + token) * a.n_q + kvh * group + head) * a.splits + split;
+            a.part_acc[slot * D + dim] = num;
+            if (dim == 0) a.part_ml[slot * 2] = base_w[n], a.part_ml[slot * 2 + 1] = sum;
+          }
+          if (++head == group) head = 0, ++token;
         }
       }
     }
@@ -473,29 +488,31 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     tmem_dealloc(tmem_base, L::TMEM);
   }
   if (a.cluster) {
-    // The splits of these rows are the cluster's CTAs: each merges every splits-th row out of the others' shared memory.
+    // The splits of these rows are the cluster's CTAs: each merges every splits-th row out of the others' shared memory, a warp a row.
     cluster_sync();
-    const uint32_t theirs = smem_base + L::OFF_K;
-    for (int e = threadIdx.x; e < N * D; e += THREADS) {
-      const int n = split + e / D * a.splits, dim = e % D;
-      if (n >= n_rows) break;
-      float acc[8], m[8], l[8], big = -INFINITY;
+    const uint32_t theirs = smem_base + L::OFF_K, at = map_to_rank(theirs, lane < a.splits ? lane : 0);
+    for (int n = split + warp * a.splits; n < n_rows; n += THREADS / 32 * a.splits) {
+      // lane i: split i's reference and sum
+      const float m = lane < a.splits ? ld_cluster_f32(at + (N * D + n) * 4) : -INFINITY, l = lane < a.splits ? ld_cluster_f32(at + (N * D + N + n) * 4) : 0.f;
+      const float big = warp_max_number(m), f = m == -INFINITY ? 0.f : fast_exp2(m - big);
+      const float den = warp_sum(f * l);      // (0 times a NaN is one: scores that are all none stay visible)
+      constexpr int EACH = D / 32;
+      float v[8][EACH], num[EACH];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ld_cluster(map_to_rank(theirs, i < a.splits ? i : 0) + (n * D + lane * EACH) * 4, v[i]);
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) num[e] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t at = map_to_rank(theirs, i < a.splits ? i : 0);
-        acc[i] = ld_cluster_f32(at + (n * D + dim) * 4), m[i] = ld_cluster_f32(at + (N * D + n) * 4), l[i] = ld_cluster_f32(at + (N * D + N + n) * 4);
-        if (i >= a.splits) m[i] = -INFINITY, l[i] = 0.f, acc[i] = 0.f;
-        big = fmaxf(big, m[i]);
-      }
-      float num = 0.f, den = 0.f;
+        const float fi = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - big);
-        num = fmaf(f, acc[i], num);
-        den = fmaf(f, l[i], den);      // (0 times a NaN is one: scores that are all none stay visible)
+        for (int e = 0; e < EACH; ++e) num[e] = i < a.splits ? fmaf(fi, v[i][e], num[e]) : num[e];
       }
       const int r = r0 + n, token = r / group, head = kvh * group + r - token * group;
-      a.out[(size_t)(qs + token) * a.out_stride + (size_t)head * D + dim] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+      __nv_bfloat16* to = a.out + (size_t)(qs + token) * a.out_stride + (size_t)head * D + lane * EACH;
+      const float inverse = den == 0.f ? 0.f : FROM_CODES / den;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) to[e] = __float2bfloat16_rn(num[e] * inverse);
     }
     cluster_sync();      // nobody's shared memory goes before the others have read it
   }

@@ -2513,9 +2513,12 @@ def q8_few_width(rows: int) -> int:
 
 
 def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
-    """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once."""
+    """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once; up to eight
+    merge inside their cluster, and up to sixteen are not worth a second kernel (16 requests of five drafted tokens over 1,700
+    keys: 23 us with eight, 29 with nine)."""
     room = (3 if width <= 16 else 2 if width <= 32 else 1) * sm_count()
-    return max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
+    splits = max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
+    return 8 if 8 < splits < 16 else splits
 
 
 def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_len: torch.Tensor, pos0: torch.Tensor,
