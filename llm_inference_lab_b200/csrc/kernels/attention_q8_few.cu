@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
   const int last = min(min(pos_hi, kvl - 1), a.max_blocks * a.page_size - 1);      // last and first key that any row sees
   const int first = lab_first_key(pos_lo, a.window);
   const int t_first = first / KEYS, all_tiles = last >= first ? last / KEYS - t_first + 1 : 0;
-  const int per_split = (all_tiles + a.splits - 1) / a.splits;
-  const int t_lo = t_first + min(all_tiles, split * per_split), n_tiles = min(all_tiles, (split + 1) * per_split) - (t_lo - t_first);
+  const int each = all_tiles / a.splits, more = all_tiles - each * a.splits;      // tiles of a split, and splits with one more
+  const int t_lo = t_first + split * each + min(split, more), n_tiles = each + (split < more ? 1 : 0);
   const int page_shift = __ffs(a.page_size) - 1;
 
   if (threadIdx.x == 0) {
