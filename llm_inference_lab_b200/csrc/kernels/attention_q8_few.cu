@@ -164,24 +164,23 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
       const int row = next;
       next = page_row(j + 1);      // looked up beside this tile's copies
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * page_bytes;
-      bool alive = mbar_wait(&bar->k_empty[s], ph ^ 1, abort_flag) && mbar_wait(&bar->v_empty[s], ph ^ 1, abort_flag);
-      if (!__all_sync(0xffffffffu, alive)) break;
-      if (lane == 0) {
-        mbar_expect_tx(&bar->k_full[s], bytes);
-        mbar_expect_tx(&bar->v_full[s], bytes);
-      }
+      // keys first: their place is free as soon as the scores are formed, the values' only after the softmax
+      if (!__all_sync(0xffffffffu, mbar_wait(&bar->k_empty[s], ph ^ 1, abort_flag))) break;
+      if (lane == 0) mbar_expect_tx(&bar->k_full[s], bytes);
       __syncwarp();
-      if (row >= 0) {
-        tma_load_2d(smem_base + L::OFF_K + s * Tile::BYTES + lane * page_bytes, &map_k, &bar->k_full[s], 0, row);
-        tma_load_2d(smem_base + L::OFF_V + s * Tile::BYTES + lane * page_bytes, &map_v, &bar->v_full[s], 0, row);
-      }
-      asked = j + 1;
+      if (row >= 0) tma_load_2d(smem_base + L::OFF_K + s * Tile::BYTES + lane * page_bytes, &map_k, &bar->k_full[s], 0, row);
+      asked = 2 * j + 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bar->v_empty[s], ph ^ 1, abort_flag))) break;
+      if (lane == 0) mbar_expect_tx(&bar->v_full[s], bytes);
+      __syncwarp();
+      if (row >= 0) tma_load_2d(smem_base + L::OFF_V + s * Tile::BYTES + lane * page_bytes, &map_v, &bar->v_full[s], 0, row);
+      asked = 2 * j + 2;
     }
-    if (asked < n_tiles) {      // a wait has run out: the copies that were asked for land before the CTA ends
+    if (asked < 2 * n_tiles) {      // a wait has run out: the copies that were asked for land before the CTA ends
       volatile int never = 0;
-      for (int j = max(0, asked - STAGES); j < asked; ++j) {
-        mbar_wait(&bar->k_full[j % STAGES], (j / STAGES) & 1, &never, 100000000ull);
-        mbar_wait(&bar->v_full[j % STAGES], (j / STAGES) & 1, &never, 100000000ull);
+      for (int i = max(0, asked - 2 * STAGES); i < asked; ++i) {
+        const int j = i / 2, s = j % STAGES;
+        mbar_wait(i & 1 ? &bar->v_full[s] : &bar->k_full[s], (j / STAGES) & 1, &never, 100000000ull);
       }
     }
   } else if (warp == 1) {
