@@ -8,7 +8,7 @@ model, dtype, input_ids, text, elapsed, ttft, generated_tokens, tok/s and
 kv_released (qwen2.rs:262-268).  Not taken over: ``--disable-overlap`` (there is
 one step in flight at a time), ``--prefix-cache`` and ``--reference-dir``
 (prefix sharing and checkpoint fixtures are out of scope).  Added:
-``--prompt-ids`` for models without a tokenizer (random weights),
+``--cache-dtype``, ``--prompt-ids`` for models without a tokenizer (random weights),
 ``--temperature`` and ``--seed``, ``--random-config`` to make a random model.
 
     python -m llm_inference_lab_b200.cli --model-dir DIR --prompt-ids 1,2,3 --max-new-tokens 8
@@ -53,6 +53,8 @@ def main(argv=None) -> int:
     ap.add_argument("--cuda-graph", action="store_true", help="replay decode steps from a CUDA graph")
     ap.add_argument("--trace-steps", action="store_true", help="one JSON line per step on stderr")
     ap.add_argument("--page-size", type=int, default=16)
+    ap.add_argument("--cache-dtype", default="auto", choices=["auto", "e4m3"],
+                    help="keys and values in the engine's type, or in 8 bits (with --dtype bf16)")
     ap.add_argument("--kv-tokens", type=int, default=None, help="size of the cache pool in tokens")
     ap.add_argument("--random-config", default=None,
                     help="a config.json: write a random model into --model-dir first (with --seed)")
@@ -82,7 +84,7 @@ def main(argv=None) -> int:
 
     t_load = time.perf_counter()
     llm = LLM(args.model_dir, args.dtype, max_batch_tokens=args.max_batch_tokens, page_size=args.page_size,
-              kv_tokens=args.kv_tokens, cuda_graph=args.cuda_graph)
+              kv_tokens=args.kv_tokens, cuda_graph=args.cuda_graph, cache_dtype=args.cache_dtype)
     if args.trace_steps:
         llm.trace = lambda rec: print(json.dumps(rec), file=sys.stderr, flush=True)
     load_s = time.perf_counter() - t_load

@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, FEW_THREADS = 64;
+constexpr int THREADS = 256, FEW_THREADS = 64, VEC_THREADS = 128;
 constexpr int MOST_DIM = 256;
 
 struct Store {
@@ -124,9 +124,10 @@ template <int N> __device__ __forceinline__ void put_codes(uint8_t* to, const fl
 
 // Whole heads rotated, d a power of two from 16 to 256 (128 for parts: a row's lanes are one warp's), everything on the boundaries of its vectors: d / (2 N) lanes a row, each
 // with N elements of its first half and the N that they turn with.  N = 8 (16 bytes of bfloat16 a load) for rows; N = 2 for
-// parts, whose steps have few rows: four times the lanes then share the sums.
+// parts, whose steps have few rows: four times the lanes then share the sums.  Blocks of 128, ten a multiprocessor (2,048 tokens of 28
+// + 8 heads of 128: 11.1 us, 12.6 by blocks of 256, four of them; the loads' latency bounds it, 3.3 TB/s).
 template <typename T, bool PARTS, int N>
-__global__ void __launch_bounds__(PARTS ? FEW_THREADS : THREADS) store_vec_kernel(const Store s) {
+__global__ void __launch_bounds__(PARTS ? FEW_THREADS : VEC_THREADS, PARTS ? 1 : 10) store_vec_kernel(const Store s) {
   pdl_trigger();
   pdl_wait();
   const int half = s.d / 2, lanes = half / N, shift = __ffs(lanes) - 1, heads = s.n_q + 2 * s.n_kv;
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(THREADS) store_any_kernel(const Store s) {
 template <typename T, bool PARTS>
 int launch_store(const Store& s, bool vec, cudaStream_t stream) {
   const long long rows = (long long)s.tokens * (s.n_q + 2 * s.n_kv);
-  constexpr int N = PARTS ? 2 : 8, threads = PARTS ? FEW_THREADS : THREADS;
+  constexpr int N = PARTS ? 2 : 8, threads = PARTS ? FEW_THREADS : VEC_THREADS;
   if (vec) {
     const long long units = rows * (s.d / (2 * N));
     return (int)lab_launch(store_vec_kernel<T, PARTS, N>, dim3((unsigned)((units + threads - 1) / threads)), dim3(threads), 0, stream, s);

@@ -65,12 +65,21 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"unknown dtype {name!r}: use bfloat16 or float32") from None
 
 
+CACHE_DTYPES = ("auto", "e4m3")
+
+
 class Engine:
-    """A model, its cache and the step function, on one GPU."""
+    """A model, its cache and the step function, on one GPU.
+
+    `cache_dtype`: "auto", keys and values in the engine's storage type; "e4m3", in 8 bits with a power of two per row (a token's
+    key or value of one kv head), half the memory of bfloat16 and half the bytes of a decode step, for bfloat16 engines of
+    models whose every cache is keys and values of mixers that take it (`Mixer.quantised_cache`)."""
 
     def __init__(self, model: CausalLM | str, dtype="bfloat16", *, max_tokens: Optional[int] = None,
                  page_size: int = 16, max_requests: int = 64, max_batch_tokens: int = 8192,
-                 max_seq_len: Optional[int] = None, device="cuda:0"):
+                 max_seq_len: Optional[int] = None, device="cuda:0", cache_dtype: str = "auto"):
+        if cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"unknown cache_dtype {cache_dtype!r}: use one of {', '.join(CACHE_DTYPES)}")
         ops.require_gpu()
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
@@ -82,6 +91,7 @@ class Engine:
         if model.dtype != self.dtype:
             raise ValueError("the model was built for another dtype than the engine")
         self.model = model
+        self.cache_dtype = cache_dtype
         bp = model.blueprint
         self.vocab = bp.vocab
         self.page_size = int(page_size)
@@ -93,6 +103,8 @@ class Engine:
         # Every request's count is rounded up to whole pages, so the pool is counted in pages.
         self.num_pages = -(-int(max_tokens) // self.page_size)
         plan = model.cache_plan
+        if cache_dtype == "e4m3":
+            self._check_quantised(model, plan)
         rt = cache_mod.runtime()
         groups = [rt.GroupConfig(self.page_size, w, self.num_pages, keep)
                   for w, keep in zip(plan.group_windows, plan.group_keeps)]
@@ -138,6 +150,9 @@ class Engine:
             return CacheView(need, group=plan.group_for(need), k=latent, block_state=block_state)
         if isinstance(need, PagedKV):
             shape = (self.num_pages, need.n_kv_heads, self.page_size, need.head_dim)
+            if self.cache_dtype == "e4m3":
+                pages = ops.quant_pages(*shape, self.device)
+                return CacheView(need, group=plan.group_for(need), pages8=pages, block_state=block_state)
             # Pages are never cleared: what may be read is decided by lengths alone.
             k = torch.empty(shape, dtype=self.dtype, device=self.device)
             v = torch.empty(shape, dtype=self.dtype, device=self.device)
@@ -146,6 +161,16 @@ class Engine:
             state = torch.zeros((self.max_requests,) + tuple(need.shape), dtype=torch.float32, device=self.device)
             return CacheView(need, state=state, block_state=block_state)
         return CacheView(None, block_state=block_state)
+
+    def _check_quantised(self, model, plan) -> None:
+        if self.dtype != torch.bfloat16:
+            raise ValueError("cache_dtype e4m3 goes with a bfloat16 engine")
+        for call in model.order:
+            need, mixer = plan.needs[call.cache], model.blocks[call.layer].mixer
+            if need is None:
+                continue
+            if not isinstance(need, PagedKV) or not getattr(mixer, "quantised_cache", False):
+                raise ValueError(f"cache_dtype e4m3: layer {call.layer}'s mixer ({type(mixer).__name__}) does not take its cache in 8 bits")
 
     @classmethod
     def _states_of(cls, view: CacheView):
@@ -197,6 +222,73 @@ class Engine:
 
     def free_pages(self) -> list[int]:
         return [self.cache.free_pages(g) for g in range(self.cache.num_groups)]
+
+    def cached_rows(self, request: int, cache: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys (as rotated) and values that one cache of the model holds of a request, in the engine's storage type: k, v
+        [tokens, n_kv, head_dim], position 0 first.  Positions whose pages were given back (a window has left them) are zeros.
+        `cache` counts the model's caches (`LayerCall.cache`)."""
+        view = self.views[cache]
+        if not isinstance(view.need, PagedKV):
+            raise ValueError(f"cache {cache} does not hold keys and values")
+        table = torch.tensor(self.cache.block_table(int(request), view.group), dtype=torch.int32, device=self.device)
+        at = torch.arange(self.cache.length(int(request)), dtype=torch.int32, device=self.device)
+        page = table[(at // self.page_size).long()]
+        slots = torch.where(page >= 0, page * self.page_size + at % self.page_size, -1)
+        if view.pages8 is not None:
+            return ops.kv_load_q8(view.pages8, slots, self.dtype)
+        rows = slots.clamp(min=0).long()
+        return tuple(torch.where((slots >= 0)[:, None, None], t[rows // self.page_size, :, rows % self.page_size], torch.zeros_like(t[:1, :, 0]))
+                     for t in (view.k, view.v))
+
+    # ------------------------------------------------------------------------------------
+    def verify_step(self, entries: Sequence[tuple], temperatures: Optional[Sequence[float]] = None,
+                    seeds: Optional[Sequence[int]] = None, draft_probs: Optional[torch.Tensor] = None) -> list[list[int]]:
+        """One step over drafted tokens: `entries` are (request, the token it goes on with, drafted tokens after it).  Every
+        request's tokens run as one short portion, the model's logits judge the drafts (`ops.verify_drafts`), and what was
+        refused leaves the cache again.  Returns each request's new tokens: the accepted drafts, and one drawn behind them, which
+        is not in the cache yet and is the token to go on with.
+
+        `temperatures` and `seeds` one per request (None: greedy); a token's draw goes by its position, as everywhere, so with
+        or without drafts a seed gives tokens of the same distribution (greedy: the same tokens).  `draft_probs`: for every
+        row of the step, in order, the probabilities that its draft was drawn from, [rows, vocab] 32-bit (a request's last row:
+        anything); None: the drafts are certain.  Models with fixed-size state are refused: it cannot go back."""
+        if self.stateful:
+            raise InvalidInput("drafted tokens: the model keeps fixed-size state, which cannot go back behind a refused token")
+        if temperatures is not None and (seeds is None or len(temperatures) != len(entries) or len(seeds) != len(entries)):
+            raise InvalidInput("drafted tokens: a temperature and a seed per request, or neither")
+        rows = [[int(token), *(int(t) for t in drafts)] for _, token, drafts in entries]
+        steps = [Entry(request, tokens, range(len(tokens))) for (request, _, _), tokens in zip(entries, rows)]
+        self.validate(steps)
+        pairs = [(int(e.request), len(e.tokens)) for e in steps]
+        began = self._begin(pairs, False)
+        try:
+            logits = self._run(steps)
+            starts, flat = [0], []
+            for tokens in rows:
+                flat += [*tokens[1:], -1]
+                starts.append(len(flat))
+            meta = torch.tensor([*flat, *starts], dtype=torch.int32).to(self.device, non_blocking=True)
+            drawn = [None, None, None]
+            if temperatures is not None:
+                held = [self.cache.length(r) + 1 for r, _ in pairs]      # the position that a request's first row decides
+                ints = torch.tensor([*(int(s) & 0x7FFFFFFF for s in seeds), *held], dtype=torch.int32).to(self.device, non_blocking=True)
+                drawn = [torch.tensor(list(temperatures), dtype=torch.float32).to(self.device, non_blocking=True), ints[: len(pairs)],
+                         ints[len(pairs):]]
+            tokens, counts = ops.verify_drafts(logits, meta[: len(flat)], meta[len(flat):], draft_probs, *drawn)
+            told = torch.cat((tokens, counts)).cpu().tolist()
+            new = [told[at: at + n] for at, n in zip(starts, told[len(flat):])]
+            for picked in new:
+                if not 0 <= picked[-1] < self.vocab:
+                    raise RuntimeError("drafted tokens: a row without any finite logit")
+        except Exception:
+            self._fail(began)
+            raise
+        for (request, _), picked in zip(pairs, new):
+            self.cache.commit(request, len(picked))
+            self.cache.rollback(request)
+        self.stats.steps += 1
+        self.stats.decode_tokens += sum(len(picked) for picked in new)
+        return new
 
     # ------------------------------------------------------------------------------------
     def validate(self, entries: Sequence[Entry], reserved: bool = False) -> None:

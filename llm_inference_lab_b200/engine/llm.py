@@ -34,9 +34,10 @@ class LLM:
     def __init__(self, model_dir: str, dtype: str = "bf16", *, max_batch_tokens: int = 512,
                  kv_tokens: Optional[int] = None, page_size: int = 16, max_requests: int = 64,
                  max_seq_len: Optional[int] = None, reserve_future: bool = True, cuda_graph: bool = False,
-                 lookahead: bool = True, device: str = "cuda:0"):
+                 lookahead: bool = True, device: str = "cuda:0", cache_dtype: str = "auto"):
         self.engine = Engine(model_dir, dtype, max_tokens=kv_tokens, page_size=page_size, max_requests=max_requests,
-                             max_batch_tokens=max_batch_tokens, max_seq_len=max_seq_len, device=device)
+                             max_batch_tokens=max_batch_tokens, max_seq_len=max_seq_len, device=device,
+                             cache_dtype=cache_dtype)
         rt = cache_mod.runtime()
         self.scheduler = rt.Scheduler(self.engine.cache, max_batch_tokens, self.engine.max_seq_len, max_requests,
                                       reserve_future)

@@ -19,9 +19,13 @@ class GQAttention(Mixer):
     Formulas: rust/engine/src/runner/model/qwen2/engine.rs:1133-1214 (projections, rotation),
     1072-1115 (cache write, attention), 1225-1232 (output projection); kv head of query
     head h is h // (n_heads / n_kv_heads) (engine.rs:1589-1617).
+    The cache may be in 8 bits (`CacheView.pages8`): keys and values are then rounded as they are written, and attended
+    as they lie.
     The three projection matrices are concatenated once at load time, so that one matrix
     product yields q, k and v.
     """
+
+    quantised_cache = True
 
     @classmethod
     def tensors(cls, spec: PartSpec):
@@ -60,6 +64,8 @@ class GQAttention(Mixer):
 
     def forward(self, x: torch.Tensor, ctx: StepContext, cache: CacheView) -> torch.Tensor:
         group = ctx.groups[cache.group]
+        if cache.pages8 is not None:
+            return self._forward8(x, ctx, cache, group)
         table_of = getattr(self.position, "table", None)
         if (table_of is not None and x.shape[0] > 128
                 and ops.qkv_fusable(x, self.w_qkv, self.d, getattr(self.position, "rotary_dim", 0))):
@@ -85,6 +91,28 @@ class GQAttention(Mixer):
             q = self.position.rotate_and_store(qkv, ctx.row_pos, group.row_slot, cache, self.n_q, self.n_kv, self.d,
                                                bias=self.b_qkv if qkv.dim() == 3 else None, scratch=ctx.scratch)
         attn = ops.attention(q, cache.k, cache.v, ctx, group, self.n_q, self.n_kv, self.d, self.window, self.scale)
+        return ops.linear(attn, self.w_o, self.b_o, allow_partial=self.b_o is None)
+
+    def _forward8(self, x: torch.Tensor, ctx: StepContext, cache: CacheView, group) -> torch.Tensor:
+        """The same over a cache in 8 bits: the store takes the projection's rows or partial products and the step's table of
+        cosines and sines; an encoding that has no table encodes the rows first."""
+        table, dims = None, 0
+        if type(self.position) is Rope:
+            qkv = ops.linear(x, self.w_qkv, self.b_qkv, allow_partial=True)
+            dims = self.position.rotary_dim
+            table = self.position.table(ctx.row_pos, ctx.scratch) if dims else None
+        else:
+            qkv = ops.linear(x, self.w_qkv, self.b_qkv)
+            self.position.encode(qkv, ctx.row_pos, self.n_q, self.n_kv, self.d)
+        slots = group.row_slot
+        if not cache.write:      # another call has written this cache: q is rotated, and nothing is stored
+            slots = ctx.scratch.get("no_slots")
+            if slots is None:
+                slots = ctx.scratch["no_slots"] = torch.full_like(group.row_slot, -1)
+        q = ops.rope_kv_store_q8(qkv, table, dims, slots, cache.pages8, self.n_q, self.n_kv, self.d,
+                                 bias=self.b_qkv if qkv.dim() == 3 else None)
+        attn = ops.attention_q8(q, cache.pages8, ctx.q_start, ctx.kv_len, ctx.pos0, group.block_table, ctx.n_requests, ctx.q_lens,
+                                ctx.max_kv_len, self.n_q, self.n_kv, self.d, self.window, self.scale)
         return ops.linear(attn, self.w_o, self.b_o, allow_partial=self.b_o is None)
 
 

@@ -72,6 +72,7 @@ class CacheView:
     write: bool = True                      # False: the call only reads what another call wrote
     k: Optional[torch.Tensor] = None        # [pages, n_kv, page_size, head_dim]; a paged latent: [pages, page_size, width]
     v: Optional[torch.Tensor] = None
+    pages8: Optional[tuple] = None          # keys and values in 8 bits instead (`ops.QuantPages`); k and v are None then
     state: Optional[torch.Tensor] = None    # [max_requests, *shape] float32
     block_state: Optional[torch.Tensor] = None   # fixed-size state of the block arrangement itself, same form
     parts: Optional[list] = None            # a need made of parts (`CacheParts`): one view per part
@@ -110,6 +111,9 @@ class Part:
 
 
 class Mixer(Part):
+    # True: the mixer also takes its paged keys and values in 8 bits (`CacheView.pages8`)
+    quantised_cache = False
+
     @classmethod
     def cache_need(cls, spec: PartSpec) -> CacheNeed:
         return None
