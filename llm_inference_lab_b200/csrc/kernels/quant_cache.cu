@@ -46,7 +46,7 @@ __device__ __forceinline__ long long pool_row(const Store& s, int token, int kv_
 }
 
 // N neighbouring numbers of a row.  PARTS: the parts are summed in 64 bits in their order, the bias added, and the sum rounded
-// once to bfloat16, the type that the rows would have.
+// to 32 bits, as a product in one piece leaves it, and then to bfloat16, the type that the rows would have.
 template <typename T, bool PARTS, int N>
 __device__ __forceinline__ void take(const Store& s, int token, int col, float (&x)[N]) {
   if constexpr (PARTS) {
@@ -78,7 +78,7 @@ __device__ __forceinline__ void take(const Store& s, int token, int col, float (
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (s.bias) sum[j] += to_f32(s.bias[col + j]);
-      x[j] = round_to<__nv_bfloat16>(q8_to_odd(sum[j]));
+      x[j] = round_to<__nv_bfloat16>((float)sum[j]);
     }
   } else {
     const T* p = static_cast<const T*>(s.rows) + (size_t)token * s.row_stride + col;

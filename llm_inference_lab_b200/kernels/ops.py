@@ -2432,7 +2432,7 @@ def rope_kv_store_q8(qkv: torch.Tensor, table: torch.Tensor | None, rotary_dim: 
     [tokens, n_q * head_dim]; `qkv` stays as it is.
 
     `qkv` is the fused projection [tokens, (n_q + 2 n_kv) * d], bfloat16 or float32, or its 32-bit partial products [parts,
-    tokens, ..] whose sum with `bias` is rounded to bfloat16 first (contiguous); `table` comes from `rope_table` (None with
+    tokens, ..] whose sum with `bias`, formed in 64 bits, is rounded to 32 and then to bfloat16 first (contiguous); `table` comes from `rope_table` (None with
     rotary_dim 0).  Slots that are not negative differ from one another.  A code is what the exact rotated number rounds to, in
     one rounding; a row with a number that is not finite reads back as NaN.  Head sizes up to 256."""
     shape, device, kind = qkv.shape, qkv.get_device(), qkv.dtype

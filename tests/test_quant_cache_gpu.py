@@ -46,9 +46,7 @@ def run_store(rng, tokens, n_q, n_kv, d, rotary_dim, page, dtype, parts=0, rows=
             b = torch.from_numpy(rng.standard_normal(width).astype(np.float32)).cuda().to(torch.bfloat16)
             total = total + b.double().cpu().numpy()
         dtype = torch.bfloat16
-        # one rounding from 64 bits to 8 significant ones
-        power = 2.0 ** (np.frexp(total)[1] - 8)
-        used = np.round(total / power) * power
+        used = torch.from_numpy(total.astype(np.float32)).to(torch.bfloat16).double().numpy()
     else:
         qkv = x.to(dtype)
         if strided:
