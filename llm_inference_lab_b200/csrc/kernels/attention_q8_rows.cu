@@ -19,13 +19,14 @@
 // alone, and none of the ways to shorten them helped: 64 keys a tile, two threads a row, fewer registers.)
 // The groups share a row's reference maximum, to which O is relative: a group decides on it for its tile after the other has
 // for the tile before, which it learns through shared memory.  The reference follows the maximum only when that has grown by
-// more than 2^8, and O is then rescaled in place, the product of the tile before being complete.  Each group keeps a sum of its own.
+// more than 2^32 (two portions of 1,024 rows: 142 us, 158 with 2^8, where some row of a warp's 32 grows in most of the first tiles;
+// no bit is lost by it, P and O being floating-point numbers), and O is then rescaled in place, the product of the tile before being complete.  Each group keeps a sum of its own.
 //
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
 //
-// Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of 168 registers become 224
-// a softmax thread and 56 the rest: 2 x 224 + 56 = 3 x 168.  Every wait is bounded.
+// Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of 168 registers become 232
+// a softmax thread and 40 the rest: 2 x 232 + 40 = 3 x 168.  Every wait is bounded.
 #include "quant8_tc.cuh"
 
 #ifndef LAB_HEAD_DIM
@@ -49,7 +50,7 @@ static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 constexpr int TM_S = 0, TM_P = GROUPS * KEYS, TM_O = TM_P + GROUPS * KEYS / 2, TMEM_COLS = 512;
 static_assert(TM_O + D <= TMEM_COLS, "tensor memory holds two S, two P and one O");
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float RESCALE = 8.f;
+constexpr float RESCALE = 32.f;      // P and O have an exponent of eight bits: up to 2^32 too large they are as exact
 
 struct Barriers {
   uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[GROUPS], s_empty[GROUPS], p_full[GROUPS],
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   const uint32_t tmem_base = bar->tmem_slot, smem_base = smem_u32(smem);
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ---------------- loader ----------------
       const int row0 = (many_before(a.q_start, b, a.fewest, lane) * a.n_kv + kvh) * a.span + (t_lo - first_tile(p0, a.window)) * KEYS;
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     }
   } else {
     // ---------------- softmax: a thread a row, a group every other tile ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int g = (warp - 4) >> 2, quarter = warp & 3, mine = quarter * 32 + lane;
     const int r = r0 + mine, token = r / group, head = kvh * group + r - token * group;
     const bool valid = r < ql * group;
