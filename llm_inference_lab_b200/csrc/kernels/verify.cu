@@ -49,6 +49,8 @@ struct Args {
   int *tokens, *counts;
 };
 
+// DRAWS false: every request is greedy.
+template <bool DRAWS>
 __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args a) {
   __shared__ float sm[STAT_THREADS / 32], ss[STAT_THREADS / 32];
   __shared__ int si[STAT_THREADS / 32];
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args 
   }
   // the row's request, looked for while its entries arrive
   float inverse = 0.f;
-  if (a.temperature != nullptr) {
+  if constexpr (DRAWS) {
     int b = 0, past = a.requests;
     while (past - b > 1) {
       const int mid = (b + past) / 2;
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args 
     const float t = a.temperature[b];
     inverse = t > 0.f ? 1.f / t : 0.f;
   }
-  const bool greedy = inverse == 0.f;
+  const bool greedy = !DRAWS || inverse == 0.f;
   float m = -INFINITY;
   int at = INT_MAX;
   if (greedy) {
@@ -93,14 +95,22 @@ __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args 
   } else {
 #pragma unroll
     for (int j = 0; j < 4 * ROUNDS; ++j) {
-      x[j] *= inverse;
-      m = fmaxf(m, x[j]);      // (a NaN is passed over)
+      x[j] = fmaxf(x[j] * inverse, -INFINITY);      // (a NaN becomes -inf, the least of all)
+      m = fmaxf(m, x[j]);
     }
   }
   float sum = 0.f;
   if (!greedy) {
+    if (fabsf(m) < INFINITY) {
 #pragma unroll
-    for (int j = 0; j < 4 * ROUNDS; ++j) sum += x[j] == m ? 1.f : x[j] == x[j] ? __expf(x[j] - m) : 0.f;
+      for (int j = 0; j < 4 * ROUNDS; ++j) sum += __expf(x[j] - m);
+    } else {      // all of them -inf, or some +inf: those that are the largest count
+#pragma unroll
+      for (int j = 0; j < 4 * ROUNDS; ++j) {
+        const int i = first + ((j >> 2) * STAT_THREADS + (int)threadIdx.x) * 4 + (j & 3);
+        sum += x[j] == m && i < end && lr[i] == lr[i] ? 1.f : 0.f;
+      }
+    }
   }
   auto join = [&](float om, float os, int oi) {
     if (greedy) {
@@ -115,9 +125,12 @@ __global__ void __launch_bounds__(STAT_THREADS) verify_chunks_kernel(const Args 
   for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (lane == 0) sm[warp] = m, ss[warp] = sum, si[warp] = at;
   __syncthreads();
-  if (threadIdx.x != 0) return;
+  if (warp != 0) return;
+  constexpr int WARPS = STAT_THREADS / 32;
+  m = sm[lane % WARPS], sum = ss[lane % WARPS], at = si[lane % WARPS];
 #pragma unroll
-  for (int w = 1; w < STAT_THREADS / 32; ++w) join(sm[w], ss[w], si[w]);
+  for (int o = WARPS / 2; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), __shfl_xor_sync(0xffffffffu, at, o));
+  if (lane != 0) return;
   a.part[(size_t)row * a.chunks + chunk] = make_float4(m, sum, __int_as_float(at), 0.f);
 }
 
@@ -283,8 +296,10 @@ __global__ void __launch_bounds__(PICK_THREADS) verify_pick_kernel(const Args a,
   if (cluster > 1) {
     cluster_sync();
     if (part != 0) return;
-    if (warp == 0)
-      for (int c = 0; c < cluster; ++c) best.join(cta_s[c]);
+    if (warp == 0) {
+      best = lane < cluster ? cta_s[lane] : Best{0.f, 0.f, INT_MAX, INT_MAX};
+      over_lanes();
+    }
   }
   if (n == 0) {
     if (threadIdx.x == 0) a.counts[b] = 0;
@@ -333,7 +348,7 @@ LAB_EXPORT int lab_verify_drafts(const LabVerify* c, cudaStream_t stream) {
   a.rows = rows, a.vocab = vocab, a.requests = requests, a.chunks = (vocab + CHUNK - 1) / CHUNK;
   a.part = (float4*)scratch, a.tokens = c->tokens, a.counts = c->counts;
   if (rows > 0) {
-    const cudaError_t e = lab_launch(verify_chunks_kernel, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
+    const cudaError_t e = lab_launch(temperature != nullptr ? verify_chunks_kernel<true> : verify_chunks_kernel<false>, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
     if (e != cudaSuccess) return (int)e;
   }
   // a cluster beyond the portable size: asked for once per device
