@@ -109,8 +109,6 @@ __global__ void __launch_bounds__(32 * WARPS) attention_q8_any_kernel(
 
 }  // namespace
 
-LAB_EXPORT int lab_attention_q8_most_dim() { return MOST_DIM; }
-
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise, both of `dtype`.  window as lab_first_key
 // takes it.
 struct LabQ8Any {

@@ -65,7 +65,8 @@ struct Args {
   long long q_stride;
   const uint8_t *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  int max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, splits, cluster;
+  int tokens, max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, longest, splits, cluster;
+  bool by_request;      // the splits' results: `longest` places a request, else one a row of the batch
   float scale_log2;
   float *part_acc, *part_ml;
 };
@@ -91,11 +92,14 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
   Barriers* bar = reinterpret_cast<Barriers*>(smem + L::OFF_BAR);
   volatile int* abort_flag = &bar->abort_flag;
   pdl_trigger();
+  // Until pdl_wait() below only the step's metadata is read (no kernel of the step writes it).
   const int b = blockIdx.z, split = blockIdx.x, group = a.n_q / a.n_kv;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   const int tiles_of_rows = gridDim.y / a.n_kv, kvh = blockIdx.y / tiles_of_rows;
   const int r0 = (blockIdx.y - kvh * tiles_of_rows) * N;       // first row: row r is token r / group, head r % group
-  if (ql > a.most_rows || r0 >= ql * group) {
+  const bool within = qs >= 0 && qs <= a.tokens - ql && ql <= a.longest;      // what the host has been told
+  if (ql > a.most_rows || r0 >= ql * group || !within) {
+    if (ql <= a.most_rows && !within && r0 == 0 && threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
     pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
     return;
   }
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
           if (a.splits == 1) {
             a.out[(size_t)(qs + token) * a.out_stride + (size_t)(kvh * group + head) * D + dim] = __float2bfloat16_rn(sum == 0.f ? 0.f : num / sum);
           } else {
-            const size_t slot = ((size_t)(qs + token) * a.n_q + kvh * group + head) * a.splits + split;
+            const size_t slot = ((size_t)((a.by_request ? b * a.longest : qs) + token) * a.n_q + kvh * group + head) * a.splits + split;
             a.part_acc[slot * D + dim] = num;
             if (dim == 0) a.part_ml[slot * 2] = base_w[n], a.part_ml[slot * 2 + 1] = sum;
           }
@@ -526,8 +530,8 @@ __global__ void __launch_bounds__(PARTS* D) attention_q8_merge_kernel(const Args
   pdl_wait();
   const int b = blockIdx.z, head = blockIdx.y, dim = threadIdx.x % D, part = threadIdx.x / D;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs, token = blockIdx.x;
-  if (ql > a.most_rows || token >= ql) return;
-  const size_t slot = ((size_t)(qs + token) * a.n_q + head) * a.splits;
+  if (ql > a.most_rows || token >= ql || qs < 0 || qs > a.tokens - ql || ql > a.longest) return;
+  const size_t slot = ((size_t)((a.by_request ? b * a.longest : qs) + token) * a.n_q + head) * a.splits;
   const int each = (a.splits + PARTS - 1) / PARTS, end = min(a.splits, (part + 1) * each);
   float big = -INFINITY, num = 0.f, den = 0.f;
   for (int s0 = part * each; s0 < end; s0 += 8) {      // eight splits' loads in flight, added in their order
@@ -600,7 +604,8 @@ int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, dim3
 
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise; requests of up to most_rows rows (longer
 // ones are left alone), `longest` the most that one of them brings; width: rows a CTA takes, 16, 32 or 48; splits of the keys, merged
-// inside their cluster (`cluster`, up to eight) or by a second kernel through scratch: tokens * n_q * splits * (D + 2) floats.
+// inside their cluster (`cluster`, up to eight) or by a second kernel through scratch: n_q * splits * (D + 2)
+// floats for each of min(tokens, requests * longest) rows.
 // window as lab_first_key takes it.
 struct LabQ8Few {
   void* out;
@@ -631,7 +636,10 @@ LAB_EXPORT int lab_attention_q8_few(const LabQ8Few* c, cudaStream_t stream) {
   a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window;
   a.most_rows = c->most_rows, a.splits = c->splits, a.cluster = c->cluster, a.scale_log2 = c->scale * LOG2E;
   const bool second = c->splits > 1 && !c->cluster;
-  a.part_acc = c->scratch, a.part_ml = second ? c->scratch + (size_t)c->tokens * c->n_q * c->splits * D : nullptr;
+  a.tokens = c->tokens, a.longest = c->longest;
+  const long long places = (long long)c->requests * c->longest;
+  a.by_request = places < c->tokens;      // (a long portion beside a few single tokens takes no place)
+  a.part_acc = c->scratch, a.part_ml = second ? c->scratch + (size_t)(a.by_request ? places : c->tokens) * c->n_q * c->splits * D : nullptr;
   const int row_tiles = (c->longest * (c->n_q / c->n_kv) + c->width - 1) / c->width;
   if ((long long)c->n_kv * row_tiles > 65535) return (int)cudaErrorInvalidValue;
   const dim3 grid(c->splits, c->n_kv * row_tiles, c->requests);

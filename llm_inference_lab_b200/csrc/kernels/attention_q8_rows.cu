@@ -20,13 +20,14 @@
 // The groups share a row's reference maximum, to which O is relative: a group decides on it for its tile after the other has
 // for the tile before, which it learns through shared memory.  The reference follows the maximum only when that has grown by
 // more than 2^32 (two portions of 1,024 rows: 142 us, 158 with 2^8, where some row of a warp's 32 grows in most of the first tiles;
-// no bit is lost by it, P and O being floating-point numbers), and O is then rescaled in place, the product of the tile before being complete.  Each group keeps a sum of its own.
+// no bit is lost by it, P and O being floating-point numbers), and O is then rescaled in place, the product of the tile before
+// being complete.  Each group keeps a sum of its own.
 //
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
 //
-// Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of 168 registers become 232
-// a softmax thread and 40 the rest: 2 x 232 + 40 = 3 x 168.  Every wait is bounded.
+// Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of
+// 168 registers become 232 a softmax thread and 40 the rest: 2 x 232 + 40 = 3 x 168.  Every wait is bounded.
 #include "quant8_tc.cuh"
 
 #ifndef LAB_HEAD_DIM
@@ -67,7 +68,7 @@ struct Args {
   long long q_stride;
   const uint8_t *k, *v, *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  int max_blocks, n_q, n_kv, page_size, num_pages, window, fewest, many;
+  int tokens, max_blocks, request0, n_q, n_kv, page_size, num_pages, window, fewest, longest, many;
   __nv_bfloat16 *wide_k, *wide_v;      // [requests of many rows][n_kv][span][D]
   int span;                            // keys, a multiple of KEYS
   float scale_log2;
@@ -75,11 +76,16 @@ struct Args {
 
 // A request's keys in scratch start at the tile of the first that its rows see.
 __device__ __forceinline__ int first_tile(int pos0, int window) { return lab_first_key(pos0, window) / KEYS; }
-// The request's number among those of many rows: by one warp, all its lanes get it.
-__device__ __forceinline__ int many_before(const int* q_start, int b, int fewest, int lane) {
+// The request's number among the launch's of many rows: by one warp, all its lanes get it.
+__device__ __forceinline__ int many_before(const Args& a, int b, int lane) {
   int n = 0;
-  for (int i = lane; i < b; i += 32) n += q_start[i + 1] - q_start[i] >= fewest;
+  for (int i = a.request0 + lane; i < b; i += 32) n += a.q_start[i + 1] - a.q_start[i] >= a.fewest;
   return __reduce_add_sync(0xffffffffu, n);
+}
+
+// Whether a request is within what the host has been told: its rows among the batch's, its keys within a request's scratch.
+__device__ __forceinline__ bool within(const Args& a, int qs, int ql, int p0, int last) {
+  return qs >= 0 && qs <= a.tokens - ql && ql <= a.longest && last < first_tile(p0, a.window) * KEYS + a.span;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -89,15 +95,19 @@ constexpr int WIDEN_THREADS = 256;
 __global__ void __launch_bounds__(WIDEN_THREADS) widen_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int ql = a.q_start[b + 1] - a.q_start[b];
+  const int b = a.request0 + blockIdx.z, kvh = blockIdx.y;
+  const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   if (ql < a.fewest) return;
   const int p0 = a.pos0[b], first = lab_first_key(p0, a.window);
   const int last = min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1;
   const int key0 = (first_tile(p0, a.window) + (int)blockIdx.x) * KEYS;
+  if (!within(a, qs, ql, p0, last)) {
+    if (threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
+    return;
+  }
   if (key0 > last) return;
   const int* bt = a.block_table + (size_t)b * a.max_blocks;
-  const int place = many_before(a.q_start, b, a.fewest, threadIdx.x & 31);
+  const int place = many_before(a, b, threadIdx.x & 31);
   if (place >= a.many) {      // more of them than the host counted: scratch has no room
     if (threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
     return;
@@ -163,15 +173,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   Barriers* bar = reinterpret_cast<Barriers*>(smem + OFF_BAR);
   volatile int* abort_flag = &bar->abort_flag;
   pdl_trigger();
+  // Until pdl_wait() below only the step's metadata is read (no kernel of the step writes it).
   // kv heads fastest, a request's last rows first: the CTAs that walk the most keys start in the first wave
-  const int b = blockIdx.z, kvh = blockIdx.x, group = a.n_q / a.n_kv;
+  const int b = a.request0 + blockIdx.z, kvh = blockIdx.x, group = a.n_q / a.n_kv;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
-  if (ql < a.fewest || r0 >= ql * group) {
+  const int p0 = a.pos0[b];
+  if (ql < a.fewest || r0 >= ql * group || !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) {
     pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
     return;
   }
-  const int p0 = a.pos0[b];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int last_row = min(r0 + ROWS, ql * group) - 1;
   const int pos_lo = p0 + r0 / group, pos_hi = p0 + last_row / group;
@@ -207,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ---------------- loader ----------------
-      const int row0 = (many_before(a.q_start, b, a.fewest, lane) * a.n_kv + kvh) * a.span + (t_lo - first_tile(p0, a.window)) * KEYS;
+      const int row0 = (many_before(a, b, lane) * a.n_kv + kvh) * a.span + (t_lo - first_tile(p0, a.window)) * KEYS;
       if (lane == 0) {
         int asked = 0;
         for (int j = 0; j < n_tiles; ++j) {
@@ -380,8 +391,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     reference[(1 + g) * ROWS] = l;
     asm volatile("bar.sync 1, 256;" ::: "memory");      // (a group that has given up comes here too)
     l += reference[(1 + (g ^ 1)) * ROWS];
-    if (ok && n_tiles > 0) {
-      ok = mbar_wait(&bar->o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, abort_flag);
+    if (n_tiles > 0) {      // (all lanes of a warp come to the vote: one that has given up may have done so alone)
+      ok = ok && mbar_wait(&bar->o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
     }
     if (ok) {      // half of the head's entries a group
@@ -391,6 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
 #pragma unroll
       for (int part = 0; part < D / 64; ++part) {
         uint32_t x[32];
+        __syncwarp();
         tmem_ld32_issue(o_addr + g * (D / 2) + part * 32, x);   // every lane takes part in the load
         tmem_wait();
         if (!valid) continue;
@@ -432,16 +444,16 @@ LAB_EXPORT long long lab_attention_q8_rows_scratch(int many, int n_kv, int windo
   return (long long)many * n_kv * span_of(window, most_keys, longest) * D * 4;
 }
 
-// A call, as the host packs it.  q: rows q_stride elements apart, on 16-byte boundaries, out likewise; requests of `fewest` rows or
-// more (shorter ones are left alone), `many` of them, `longest` the most rows that one brings; lengths are at most most_keys;
-// scratch on a boundary of 16 bytes.  window as lab_first_key takes it.
+// A call, as the host packs it.  q: `tokens` rows q_stride elements apart, on 16-byte boundaries, out likewise; the `requests` from
+// request0 on, those of `fewest` rows or more (shorter ones are left alone), `many` of them, `longest` the most rows that one
+// brings; lengths are at most most_keys; scratch on a boundary of 16 bytes.  window as lab_first_key takes it.
 struct LabQ8Rows {
   void* out;
   const void *q, *k, *v, *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
   void* scratch;
   long long out_stride, q_stride;
-  int max_blocks, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys;
+  int tokens, max_blocks, request0, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys;
   float scale;
 };
 
@@ -449,7 +461,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   if (c->requests <= 0 || c->longest <= 0 || c->many <= 0) return 0;
   const int span = span_of(c->window, c->most_keys, c->longest);
   const long long rows = (long long)c->many * c->n_kv * span;
-  if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->max_blocks < 1 || c->num_pages < 1 || c->fewest < 1 || c->page_size < 1 ||
+  if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->max_blocks < 1 || c->num_pages < 1 || c->fewest < 1 || c->page_size < 1 || c->request0 < 0 ||
       c->most_keys < 1 || rows >= (1ll << 31) || c->requests > 65535 || c->n_kv > 65535 || c->q_stride % 8 || (((uintptr_t)c->q) & 15) ||
       ((((uintptr_t)c->k) | ((uintptr_t)c->v) | ((uintptr_t)c->scratch)) & 15) || c->scratch == nullptr)
     return (int)cudaErrorInvalidValue;
@@ -458,7 +470,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   a.k = (const uint8_t*)c->k, a.v = (const uint8_t*)c->v, a.k_scale = (const uint8_t*)c->k_scale, a.v_scale = (const uint8_t*)c->v_scale;
   a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
   a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window, a.fewest = c->fewest;
-  a.many = c->many, a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
+  a.tokens = c->tokens, a.request0 = c->request0, a.longest = c->longest, a.many = c->many, a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
   a.scale_log2 = c->scale * LOG2E;
   CUtensorMap mk, mv;
   int rc;

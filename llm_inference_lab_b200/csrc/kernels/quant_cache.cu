@@ -122,10 +122,11 @@ template <int N> __device__ __forceinline__ void put_codes(uint8_t* to, const fl
     *reinterpret_cast<uint16_t*>(to) = (uint16_t)q8_encode2(x[0] * inverse, x[1] * inverse);
 }
 
-// Whole heads rotated, d a power of two from 16 to 256 (128 for parts: a row's lanes are one warp's), everything on the boundaries of its vectors: d / (2 N) lanes a row, each
-// with N elements of its first half and the N that they turn with.  N = 8 (16 bytes of bfloat16 a load) for rows; N = 2 for
-// parts, whose steps have few rows: four times the lanes then share the sums.  Blocks of 128, ten a multiprocessor (2,048 tokens of 28
-// + 8 heads of 128: 11.1 us, 12.6 by blocks of 256, four of them; the loads' latency bounds it, 3.3 TB/s).
+// Whole heads rotated, d a power of two from 16 to 256 (128 for parts: a row's lanes are one warp's), everything on the boundaries
+// of its vectors: d / (2 N) lanes a row, each with N elements of its first half and the N that they turn with.  N = 8 (16 bytes of
+// bfloat16 a load) for rows; N = 2 for parts, whose steps have few rows: four times the lanes then share the sums.  Blocks of 128,
+// ten a multiprocessor (2,048 tokens of 28 + 8 heads of 128: 11.1 us, 12.6 by blocks of 256, four of them; the loads' latency
+// bounds it, 3.3 TB/s).
 template <typename T, bool PARTS, int N>
 __global__ void __launch_bounds__(PARTS ? FEW_THREADS : VEC_THREADS, PARTS ? 1 : 10) store_vec_kernel(const Store s) {
   pdl_trigger();
@@ -338,10 +339,8 @@ int launch_load(T* out_k, T* out_v, const uint8_t* k, const uint8_t* v, const ui
 
 }  // namespace
 
-LAB_EXPORT int lab_q8_most_dim() { return MOST_DIM; }
-
 // A call, as the host packs it.  rows: [tokens, row_stride] of `dtype`, or (parts > 0) [parts, tokens, width] floats whose sum with
-// `bias` is rounded to bfloat16 first; width = (n_q + 2 n_kv) d.  table: [tokens, rotary_dim / 2] (cos, sin).  q_out: [tokens, n_q *
+// `bias` is rounded to 32 bits and then to bfloat16 first; width = (n_q + 2 n_kv) d.  table: [tokens, rotary_dim / 2] (cos, sin).  q_out: [tokens, n_q *
 // d].  Slots that are not negative differ from one another.
 struct LabQ8Store {
   const void *rows, *bias, *table;

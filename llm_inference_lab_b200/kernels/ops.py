@@ -2364,7 +2364,7 @@ _pack_store = struct.Struct("9P2q9i").pack
 _pack_load = struct.Struct("7Pq5i").pack
 _pack_any = struct.Struct("10P2q10if").pack
 _pack_few = struct.Struct("11P2q13if").pack
-_pack_rows = struct.Struct("11P2q11if").pack
+_pack_rows = struct.Struct("11P2q13if").pack
 _pack_verify = struct.Struct("10P2q3i").pack
 
 
@@ -2432,8 +2432,8 @@ def rope_kv_store_q8(qkv: torch.Tensor, table: torch.Tensor | None, rotary_dim: 
     [tokens, n_q * head_dim]; `qkv` stays as it is.
 
     `qkv` is the fused projection [tokens, (n_q + 2 n_kv) * d], bfloat16 or float32, or its 32-bit partial products [parts,
-    tokens, ..] whose sum with `bias`, formed in 64 bits, is rounded to 32 and then to bfloat16 first (contiguous); `table` comes from `rope_table` (None with
-    rotary_dim 0).  Slots that are not negative differ from one another.  A code is what the exact rotated number rounds to, in
+    tokens, ..] whose sum with `bias`, formed in 64 bits, is rounded to 32 and then to bfloat16 first (contiguous); `table` comes
+    from `rope_table` (None with rotary_dim 0).  Slots that are not negative differ from one another.  A code is what the exact rotated number rounds to, in
     one rounding; a row with a number that is not finite reads back as NaN.  Head sizes up to 256."""
     shape, device, kind = qkv.shape, qkv.get_device(), qkv.dtype
     parts = shape[0] if len(shape) == 3 else 0
@@ -2503,6 +2503,9 @@ def _refuse_load(pages, slots, dtype):
     _place(what, slots, *pages)
 
 
+# Scratch of one launch over requests of many rows: those that need more go in several, one after the other (with one request at
+# least), so that many portions beside one long context do not take memory for its length each.
+Q8_WIDE_BYTES = 1 << 30
 # Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, which splits the keys.
 Q8_FEW_ROWS = 128
 
@@ -2531,11 +2534,15 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
 
     bfloat16 queries of heads of 64 and 128 over pages of 8 to 128 (a power of two) run on the tensor cores; 32-bit queries (in
     32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `Q8_FEW_ROWS` rows
-    and query heads of a kv head take scratch for their keys and values in bfloat16, as many as their rows see."""
+    and query heads of a kv head take scratch for their keys and values in bfloat16, `max_kv_len` of them or what a window leaves,
+    up to `Q8_WIDE_BYTES` at a time.  A request beyond `q_lens`, the rows of q or `max_kv_len` is reported (`take_device_errors`)
+    where a kernel's work is sized by them, and its rows stay as they are."""
     k, v, ks, vs = pages
     device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
-    if not (q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1 and (kind is torch.bfloat16 or kind is torch.float32)
-            and n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256 and scale > 0 and len(q_lens) == n_requests
+    shape = q.shape
+    if not (len(shape) == 2 and shape[1] == width and q.stride(1) == 1 and (kind is torch.bfloat16 or kind is torch.float32)
+            and n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256 and scale > 0 and len(q_lens) == n_requests
+            and sum(q_lens) <= shape[0] and min(q_lens, default=0) >= 0
             and len(table_shape) == 2 and table_shape[0] >= n_requests and device >= 0 and device == _device_now()
             and _pages_fit(pages, device, n_kv, head_dim) and _ints_fit(q_start, device, n_requests + 1) and _ints_fit(kv_len, device, n_requests)
             and _ints_fit(pos0, device, n_requests) and _ints_fit(block_table, device, 0)
@@ -2564,10 +2571,13 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
         L.lab_attention_q8_rows_scratch.restype = ctypes.c_longlong
         many = sum(1 for n in q_lens if n > few)
-        scratch = torch.empty((int(L.lab_attention_q8_rows_scratch(many, n_kv, window, max_kv_len, longest)),), dtype=_BYTE, device=q.device)
-        _check(_entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)(_pack_rows(
-            *tensors, scratch.data_ptr(), out.stride(0), stride, blocks, n_requests, n_q, n_kv, page_size, num_pages, window, few + 1, longest,
-            many, max_kv_len, scale), stream), "attention_q8", 2)
+        each = int(L.lab_attention_q8_rows_scratch(1, n_kv, window, max_kv_len, longest))
+        at_once = max(1, min(many, Q8_WIDE_BYTES // each))
+        scratch = torch.empty((at_once * each,), dtype=_BYTE, device=q.device)
+        for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < many else ((0, n_requests, many),):
+            _check(_entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)(_pack_rows(
+                *tensors, scratch.data_ptr(), out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
+                few + 1, longest, held, max_kv_len, scale), stream), "attention_q8", 2)
     if longest_few:
         wide = q8_few_width(longest_few * group)
         if longest_few == 1 and longest == 1:
@@ -2576,11 +2586,27 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             ctas = n_kv * sum(-(-n * group // wide) for n in q_lens if n <= few)
         splits = q8_few_splits(ctas, wide, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few))
         cluster = 2 <= splits <= 8
-        scratch = torch.empty((tokens * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device) if splits > 8 else None
+        scratch = None
+        if splits > 8:
+            places = min(tokens, n_requests * longest_few)
+            scratch = torch.empty((places * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device)
         _check(_entry("attention_q8_few", "lab_attention_q8_few", head_dim)(_pack_few(
             *tensors, scratch.data_ptr() if scratch is not None else 0, out.stride(0), stride, tokens, blocks, n_requests, n_q, n_kv, page_size,
             num_pages, window, few, longest_few, wide, splits, cluster, scale), stream), "attention_q8", 1 if scratch is None else 2)
     return out
+
+
+def _spans_of_many(q_lens, few: int, at_once: int) -> list[tuple[int, int, int]]:
+    """The requests cut into runs (first, behind the last, requests of more than `few` rows) with `at_once` such at most."""
+    runs, first, held = [], 0, 0
+    for b, n in enumerate(q_lens):
+        if n > few:
+            if held == at_once:
+                runs.append((first, b, held))
+                first, held = b, 0
+            held += 1
+    runs.append((first, len(q_lens), held))
+    return runs
 
 
 def _refuse_attention(q, pages, q_start, kv_len, pos0, block_table, n_requests, q_lens, n_q, n_kv, head_dim, scale, out):
@@ -2588,13 +2614,14 @@ def _refuse_attention(q, pages, q_start, kv_len, pos0, block_table, n_requests, 
     _refuse_pages(what, pages, n_kv, head_dim)
     width = n_q * head_dim
     _require(q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1, f"{what}: q of {width} neighbouring numbers a row, got {tuple(q.shape)}")
-    _require(n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
+    _require(n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
     _require(scale > 0, f"{what}: the scale is positive")
     for name, t, count in (("q_start", q_start, n_requests + 1), ("kv_len", kv_len, n_requests), ("pos0", pos0, n_requests)):
         _refuse_ints(what, name, t, count)
     _refuse_ints(what, "block_table", block_table, 0)
     _require(block_table.dim() == 2 and block_table.shape[0] >= n_requests, f"{what}: a row of the block table per request")
     _require(len(q_lens) == n_requests, f"{what}: the host's row counts, one per request")
+    _require(sum(q_lens) <= q.shape[0] and min(q_lens, default=0) >= 0, f"{what}: row counts within the {q.shape[0]} rows of q")
     _require(out is None or (out.dtype == q.dtype and out.shape == q.shape and out.stride(1) == 1), f"{what}: out as q")
     dtype_code(q.dtype)
     _place(what, q, q_start, kv_len, pos0, block_table, out, *pages)
@@ -2617,7 +2644,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tens
     token a request's first row decides; no temperature, or 0: greedy.  Emitted tokens are distributed as the target's own.
 
     Returns (tokens [rows], counts [requests]), int32: counts[b] tokens from row starts[b] on, drafts that were accepted and then
-    the drawn one, -1 behind them.  A row without any number gives INT32_MAX, as `sample` does."""
+    the drawn one, -1 behind them; rows of no request hold nothing.  A row without any number gives INT32_MAX, as `sample` does."""
     shape, device, requests = logits.shape, logits.get_device(), starts.numel() - 1
     if not (len(shape) == 2 and logits.dtype is torch.float32 and logits.stride(1) == 1 and 0 < shape[1] and shape[0] <= 65535 and device >= 0
             and device == _device_now() and _ints_fit(drafts, device, shape[0]) and _ints_fit(starts, device, 1)

@@ -244,3 +244,61 @@ def test_two_ways_agree_on_stored_rows():
         # p's two codes (2^-8 and a sixteenth of that for their floor in a tile), the result's rounding
         slack = 2.0 ** -8 * 1.1 * torch.einsum("tkgj,jkd->tkgd", p, v.abs()) + 2.0 ** -8 * want.abs() + 2.0 ** -12 * v.abs().max()
         assert ((out - want).abs() <= slack).all()
+
+
+def test_long_portions_in_several_launches(monkeypatch):
+    """Scratch for one long request at a time: the bits of a launch over all of them."""
+    rng = np.random.default_rng(14)
+    batch = Batch(rng, [150, 1, 200, 0, 7, 140], [30, 300, 0, 5, 60, 500], 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 64)
+    x = torch.randn((batch.tokens, 8 * 64), device="cuda").to(torch.bfloat16)
+    call = lambda: ops.attention_q8(x, pages, *batch.args(), 8, 2, 64, 0, 0.125)  # noqa: E731
+    together = call()
+    monkeypatch.setattr(ops, "Q8_WIDE_BYTES", 1)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    apart = call()
+    taken = torch.cuda.max_memory_allocated() - before
+    ops.take_device_errors()
+    assert torch.equal(together, apart)
+    one = 2 * (640 // 128 + 1) * 128 * 64 * 4          # kv heads, 640 keys and a tile, keys and values in bfloat16
+    assert taken <= one + apart.nbytes + 2 ** 21       # (the splits of the few rows and the batch's numbers: far below 2 MB)
+
+
+def test_a_long_portion_beside_a_single_token_takes_no_place_for_splits():
+    """Many splits of one row's keys: their results are counted in rows of such requests, not in rows of the batch."""
+    rng = np.random.default_rng(15)
+    n_q, n_kv, d, page = 8, 2, 64, 16
+    batch = Batch(rng, [1, 1500], [20000, 0], page)
+    pages = random_pages(ops, rng, batch.num_pages, n_kv, page, d)
+    args = batch.args()
+    splits = ops.q8_few_splits(n_kv * 1, 16, 20001)
+    assert splits > 16
+    x = torch.randn((batch.tokens, n_q * d), device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = ops.attention_q8(x, pages, *args, n_q, n_kv, d, 0, d ** -0.5)
+    taken = torch.cuda.max_memory_allocated() - before
+    ops.take_device_errors()
+    wide = n_kv * (20096 // 128 + 1) * 128 * d * 4
+    assert taken <= out.nbytes + wide + 2 * n_q * splits * (d + 2) * 4 + 2 ** 20
+    alone = ops.attention_q8(x[:1], pages, args[0][:2].contiguous(), args[1][:1], args[2][:1], args[3][:1], 1, [1], 20001, n_q, n_kv, d, 0, d ** -0.5)
+    assert torch.equal(out[:1], alone)
+
+
+@pytest.mark.parametrize("told, rows, keys, most", [
+    (1, 5, 5, 5), (5, 9, 9, 9),                      # more rows than the host's count, and than q has
+    (200, 300, 300, 300), (200, 200, 900, 300),      # portions: more rows, and more keys than `max_kv_len`
+])
+def test_requests_beyond_what_the_host_said_are_reported(told, rows, keys, most):
+    rng = np.random.default_rng(16)
+    batch = Batch(rng, [rows], [keys - rows], 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 64)
+    q_start, kv_len, pos0, table, *_ = batch.args()
+    q = torch.ones((told, 4 * 64), dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, 1, [told], most, 4, 2, 64, 0, 0.125, out=out)
+    with pytest.raises(ops.KernelError, match="row"):
+        ops.take_device_errors()
+    assert (out == 7.0).all()

@@ -127,3 +127,26 @@ def test_splits_leave_no_cta_without_room_or_keys(ctas, keys):
 @pytest.mark.parametrize("rows", [1, 7, 16, 17, 32, 33, 48, 49, 1000])
 def test_widths_are_built(rows):
     assert ops.q8_few_width(rows) in (16, 32, 48) and (rows > 48 or ops.q8_few_width(rows) >= rows)
+
+
+@pytest.mark.parametrize("change, says", [
+    (dict(q_lens=[3, 1]), "row counts within the 3 rows"),
+    (dict(q_lens=[4, -1]), "row counts within the 3 rows"),
+    (dict(n_q=0, q=torch.zeros((3, 0), dtype=torch.bfloat16)), "0 query heads"),
+])
+def test_attention_refuses_rows_and_heads_that_are_not_there(change, says):
+    a = dict(q=torch.zeros((3, 6 * 64), dtype=torch.bfloat16), pages=pages(), q_start=ints(0, 2, 3), kv_len=ints(2, 1), pos0=ints(0, 0),
+             block_table=torch.zeros((2, 3), dtype=torch.int32), n_requests=2, q_lens=[2, 1], max_kv_len=2, n_q=6, n_kv=2, head_dim=64,
+             window=0, scale=0.125)
+    a.update(change)
+    with pytest.raises(KERNEL_ERROR, match=says):
+        ops.attention_q8(**a)
+
+
+@pytest.mark.parametrize("q_lens", [[200], [1, 200, 1], [200, 300, 1, 0, 129, 500, 2], [129] * 7])
+@pytest.mark.parametrize("at_once", [1, 2, 3])
+def test_runs_of_long_requests_cover_each_request_once(q_lens, at_once):
+    runs = ops._spans_of_many(q_lens, 128, at_once)
+    assert [b for first, end, _ in runs for b in range(first, end)] == list(range(len(q_lens)))
+    for first, end, held in runs:
+        assert held == sum(n > 128 for n in q_lens[first:end]) and 1 <= held <= at_once
