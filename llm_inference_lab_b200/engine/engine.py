@@ -171,6 +171,8 @@ class Engine:
                 continue
             if not isinstance(need, PagedKV) or not getattr(mixer, "quantised_cache", False):
                 raise ValueError(f"cache_dtype e4m3: layer {call.layer}'s mixer ({type(mixer).__name__}) does not take its cache in 8 bits")
+            if need.head_dim > ops.Q8_MOST_HEAD_DIM:
+                raise ValueError(f"cache_dtype e4m3: layer {call.layer}'s heads of {need.head_dim}, up to {ops.Q8_MOST_HEAD_DIM} are taken")
 
     @classmethod
     def _states_of(cls, view: CacheView):

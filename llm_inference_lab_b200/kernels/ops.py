@@ -2359,6 +2359,7 @@ def quant_pages(num_pages: int, n_kv: int, page_size: int, head_dim: int, device
 # arguments one by one cost the host 9 microseconds, a record 3.5.  Likewise an operator looks at its arguments in one expression,
 # and only where that does not hold goes through them again to say which it is.
 _E4M3, _BYTE, _INT = torch.float8_e4m3fn, torch.uint8, torch.int32
+Q8_MOST_HEAD_DIM = 256
 _device_now = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _pack_store = struct.Struct("9P2q9i").pack
 _pack_load = struct.Struct("7Pq5i").pack
@@ -2439,7 +2440,7 @@ def rope_kv_store_q8(qkv: torch.Tensor, table: torch.Tensor | None, rotary_dim: 
     parts = shape[0] if len(shape) == 3 else 0
     tokens, width = shape[-2] if len(shape) > 1 else 0, (n_q + 2 * n_kv) * head_dim
     k, v, ks, vs = pages
-    if not (2 <= len(shape) <= 3 and shape[-1] == width and 0 <= rotary_dim <= head_dim <= 256 and rotary_dim % 2 == 0 and device >= 0
+    if not (2 <= len(shape) <= 3 and shape[-1] == width and 0 <= rotary_dim <= head_dim <= Q8_MOST_HEAD_DIM and rotary_dim % 2 == 0 and device >= 0
             and device == _device_now() and _ints_fit(slots, device, tokens) and _pages_fit(pages, device, n_kv, head_dim)
             and (qkv.is_contiguous() and kind is torch.float32 if parts else len(shape) == 2 and qkv.stride(1) == 1 and
                  (kind is torch.bfloat16 or kind is torch.float32))
@@ -2467,7 +2468,7 @@ def _refuse_store(qkv, table, rotary_dim, slots, pages, n_q, n_kv, head_dim, bia
     _require(qkv.dim() == 2 or (parts > 0 and qkv.dtype == torch.float32 and qkv.is_contiguous()), f"{what}: partial products are contiguous float32")
     _require(bias is None or (parts > 0 and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == width),
              f"{what}: a bias of {width} bfloat16 numbers goes with partial products")
-    _require(0 <= rotary_dim <= head_dim <= 256 and rotary_dim % 2 == 0, f"{what}: head size {head_dim} up to 256, rotary_dim {rotary_dim} even")
+    _require(0 <= rotary_dim <= head_dim <= Q8_MOST_HEAD_DIM and rotary_dim % 2 == 0, f"{what}: head size {head_dim} up to {Q8_MOST_HEAD_DIM}, rotary_dim {rotary_dim} even")
     _require(rotary_dim == 0 or (table is not None and table.dtype == torch.float32 and table.is_contiguous()
                                  and tuple(table.shape) == (tokens, rotary_dim // 2, 2)),
              f"{what}: a table [{tokens}, {rotary_dim // 2}, 2] of cosines and sines, float32 and contiguous")
@@ -2541,7 +2542,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
     shape = q.shape
     if not (len(shape) == 2 and shape[1] == width and q.stride(1) == 1 and (kind is torch.bfloat16 or kind is torch.float32)
-            and n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256 and scale > 0 and len(q_lens) == n_requests
+            and n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= Q8_MOST_HEAD_DIM and scale > 0 and len(q_lens) == n_requests
             and sum(q_lens) <= shape[0] and min(q_lens, default=0) >= 0
             and len(table_shape) == 2 and table_shape[0] >= n_requests and device >= 0 and device == _device_now()
             and _pages_fit(pages, device, n_kv, head_dim) and _ints_fit(q_start, device, n_requests + 1) and _ints_fit(kv_len, device, n_requests)
@@ -2614,7 +2615,7 @@ def _refuse_attention(q, pages, q_start, kv_len, pos0, block_table, n_requests, 
     _refuse_pages(what, pages, n_kv, head_dim)
     width = n_q * head_dim
     _require(q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1, f"{what}: q of {width} neighbouring numbers a row, got {tuple(q.shape)}")
-    _require(n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= 256, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
+    _require(n_q >= n_kv > 0 and n_q % n_kv == 0 and head_dim <= Q8_MOST_HEAD_DIM, f"{what}: {n_q} query heads over {n_kv} kv heads of {head_dim}")
     _require(scale > 0, f"{what}: the scale is positive")
     for name, t, count in (("q_start", q_start, n_requests + 1), ("kv_len", kv_len, n_requests), ("pos0", pos0, n_requests)):
         _refuse_ints(what, name, t, count)

@@ -150,3 +150,19 @@ def test_runs_of_long_requests_cover_each_request_once(q_lens, at_once):
     assert [b for first, end, _ in runs for b in range(first, end)] == list(range(len(q_lens)))
     for first, end, held in runs:
         assert held == sum(n > 128 for n in q_lens[first:end]) and 1 <= held <= at_once
+
+
+@pytest.mark.parametrize("head_dim, taken", [(256, True), (272, False)])
+def test_engine_refuses_heads_that_no_kernel_takes(head_dim, taken):
+    from types import SimpleNamespace as Some
+
+    from llm_inference_lab_b200.engine.engine import Engine
+    from llm_inference_lab_b200.parts.spec import PagedKV
+    model = Some(order=[Some(layer=0, cache=0)], blocks=[Some(mixer=Some(quantised_cache=True))])
+    plan = Some(needs=[PagedKV(n_kv_heads=1, head_dim=head_dim)])
+    check = lambda: Engine._check_quantised(Some(dtype=torch.bfloat16), model, plan)  # noqa: E731
+    if taken:
+        check()
+    else:
+        with pytest.raises(ValueError, match="heads of 272"):
+            check()
