@@ -83,6 +83,27 @@ __device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[4]) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
 
+// Sums of M rows' values (16 or 32) over a warp: lanes halve the rows between them, 16 exchanges for 16 rows and 31 for 32, five a
+// row otherwise (16 requests of five drafted tokens: 13.4 us, 13.9).  Lane i gets row i * M / 32.
+template <int M> __device__ __forceinline__ float warp_row_sums(const float* v, int lane) {
+  float x[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) x[i] = v[i];
+  int o = 16;
+#pragma unroll
+  for (int half = M / 2; half > 0; half /= 2, o /= 2) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float give = upper ? x[i] : x[i + half], keep = upper ? x[i + half] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (int rest = 16 / M; rest > 0; rest /= 2) x[0] += __shfl_xor_sync(0xffffffffu, x[0], rest);
+  return x[0];
+}
+
 template <int N>
 __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attention_q8_few_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const Args a) {
@@ -451,13 +472,13 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
     asm volatile("bar.sync 2, 128;" ::: "memory");      // (the last tile's exponents have been read)
 #pragma unroll
     for (int n0 = 0; n0 < N; n0 += 32) {
-      float own = 0.f;
-#pragma unroll
-      for (int n = 0; n < 32 && n0 + n < N; ++n) {
-        const float s = warp_sum(l[n0 + n]);
-        if (lane == n) own = s;
+      constexpr int LAST = N % 32 == 0 ? 32 : 16;
+      if (n0 + 32 <= N) {
+        sums[(n0 + lane) * 4 + w] = warp_row_sums<32>(l + n0, lane);
+      } else {
+        const float own = warp_row_sums<LAST>(l + n0, lane);
+        if (lane % (32 / LAST) == 0) sums[(n0 + lane * LAST / 32) * 4 + w] = own;
       }
-      if (n0 + lane < N) sums[(n0 + lane) * 4 + w] = own;
       if (n0 + lane < N) base_w[n0 + lane] = n0 == 0 ? ref : ref2;
     }
     asm volatile("bar.sync 2, 128;" ::: "memory");
