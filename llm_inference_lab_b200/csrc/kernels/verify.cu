@@ -12,8 +12,8 @@
 // exact arithmetic only where two numbers agree to about 2^-20.
 //
 // Two launches: the rows' largest entry and sum of exponentials by chunk (every logit read once: the bound, memory), then a
-// cluster of sixteen CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that is
-// left (its logits come from L2).  Partial results lie in the caller's scratch and nothing has to be zero before a call, so calls
+// cluster of sixteen or four CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that
+// is left (its logits come from L2).  Partial results lie in the caller's scratch and nothing has to be zero before a call, so calls
 // on several streams, or from several graphs, do not meet.
 #include <limits.h>
 
@@ -346,8 +346,11 @@ LAB_EXPORT int lab_verify_drafts(const LabVerify* c, cudaStream_t stream) {
     const cudaError_t e = lab_launch(temperature != nullptr ? verify_chunks_kernel<true> : verify_chunks_kernel<false>, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);
     if (e != cudaSuccess) return (int)e;
   }
+  // Draws: sixteen CTAs a request while all of them find room, four beyond that, where each CTA's start is paid in turns (rows of
+  // 151,936, five a request; 12 requests 19.2 us by sixteen and 23.6 by four, 18: 27.4 and 26.6, 48: 63 and 52, 128: 157 and 114;
+  // by two 106 at 128, but 54 at 48).
+  const int cluster = temperature == nullptr ? 1 : (long long)requests * CLUSTER <= 2 * lab_sm_count() ? CLUSTER : CLUSTER / 4;
   // a cluster beyond the portable size: asked for once per device
-  const int cluster = temperature != nullptr ? CLUSTER : 1;
   static std::atomic<bool> allowed[LabShared::kDevices] = {};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
