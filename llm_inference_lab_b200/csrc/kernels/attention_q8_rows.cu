@@ -26,6 +26,9 @@
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
 //
+// Where the rows make fewer CTAs than the GPU holds (a portion of a few hundred rows behind a long context), the keys are split over
+// CTAs: each leaves its O, reference and sum in scratch, and a third kernel joins them.
+//
 // Warps: 0 loads (TMA), 1 issues the scores' products, 2 those with V, 4-7 and 8-11 are the groups.  setmaxnreg: 384 threads of
 // 168 registers become 232 a softmax thread and 40 the rest: 2 x 232 + 40 = 3 x 168.  Every wait is bounded.
 #include "quant8_tc.cuh"
@@ -71,6 +74,8 @@ struct Args {
   int tokens, max_blocks, request0, n_q, n_kv, page_size, num_pages, window, fewest, longest, many;
   __nv_bfloat16 *wide_k, *wide_v;      // [requests of many rows][n_kv][span][D]
   int span;                            // keys, a multiple of KEYS
+  int splits;                          // of the keys of a tile of rows
+  float* part;                         // of a split: [D + 2][ROWS], the entries of O, the reference and the sum of each row
   float scale_log2;
 };
 
@@ -86,6 +91,11 @@ __device__ __forceinline__ int many_before(const Args& a, int b, int lane) {
 // Whether a request is within what the host has been told: its rows among the batch's, its keys within a request's scratch.
 __device__ __forceinline__ bool within(const Args& a, int qs, int ql, int p0, int last) {
   return qs >= 0 && qs <= a.tokens - ql && ql <= a.longest && last < first_tile(p0, a.window) * KEYS + a.span;
+}
+
+// Where a split of a tile of rows leaves its results: `tiles` tiles a request and kv head.
+__device__ __forceinline__ float* part_of(const Args& a, int place, int tile, int tiles, int kvh, int split) {
+  return a.part + ((((size_t)place * tiles + tile) * a.n_kv + kvh) * a.splits + split) * ((D + 2) * ROWS);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -175,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   pdl_trigger();
   // Until pdl_wait() below only the step's metadata is read (no kernel of the step writes it).
   // kv heads fastest, a request's last rows first: the CTAs that walk the most keys start in the first wave
-  const int b = a.request0 + blockIdx.z, kvh = blockIdx.x, group = a.n_q / a.n_kv;
+  const int b = a.request0 + blockIdx.z, split = blockIdx.x / a.n_kv, kvh = blockIdx.x - split * a.n_kv, group = a.n_q / a.n_kv;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
   const int p0 = a.pos0[b];
@@ -189,7 +199,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   const int last_row = min(r0 + ROWS, ql * group) - 1;
   const int pos_lo = p0 + r0 / group, pos_hi = p0 + last_row / group;
   const int last = min(min(pos_hi, a.kv_len[b] - 1), a.max_blocks * a.page_size - 1), first = lab_first_key(pos_lo, a.window);
-  const int t_lo = first / KEYS, n_tiles = last >= first ? last / KEYS - t_lo + 1 : 0;
+  const int all_tiles = last >= first ? last / KEYS - first / KEYS + 1 : 0, each = all_tiles / a.splits, more = all_tiles - each * a.splits;
+  const int t_lo = first / KEYS + split * each + min(split, more), n_tiles = each + (split < more ? 1 : 0);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -397,7 +408,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
       ok = ok && mbar_wait(&bar->o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok) {      // half of the head's entries a group
+    if (ok && a.splits > 1) {      // half of the head's entries a group, neighbouring rows side by side
+      tc_fence_after();
+      const int place = many_before(a, b, lane);
+      const bool room = place < a.many;      // (more of them than the host counted: the first kernel has reported it)
+      float* to = part_of(a, room ? place : 0, gridDim.y - 1 - blockIdx.y, gridDim.y, kvh, split) + mine;
+#pragma unroll
+      for (int part = 0; part < D / 64; ++part) {
+        uint32_t x[32];
+        tmem_ld32_issue(o_addr + g * (D / 2) + part * 32, x);
+        tmem_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (room) to[(g * (D / 2) + part * 32 + i) * ROWS] = n_tiles == 0 ? 0.f : __uint_as_float(x[i]);
+      }
+      if (g == 0 && room) to[D * ROWS] = n_tiles == 0 ? -INFINITY : *reference, to[(D + 1) * ROWS] = l;
+    } else if (ok) {      // half of the head's entries a group
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + (size_t)(qs + token) * a.out_stride + (size_t)head * D + g * (D / 2);
@@ -432,6 +458,50 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   }
 }
 
+// The splits of a tile of rows put together: a thread a row and MERGED entries of the head, neighbouring threads neighbouring rows, 16
+// bytes a store (two portions of 256 rows over 3,000 keys in three: 33 us with the call's other kernels, 59 with 2 bytes a store).
+constexpr int MERGED = 8;
+__global__ void __launch_bounds__(ROWS, 6) attention_q8_rows_merge_kernel(const Args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = a.request0 + blockIdx.z, piece = blockIdx.x / a.n_kv, kvh = blockIdx.x - piece * a.n_kv, group = a.n_q / a.n_kv;
+  const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs, p0 = a.pos0[b], r = blockIdx.y * ROWS + threadIdx.x;
+  if (ql < a.fewest || (int)blockIdx.y * ROWS >= ql * group ||
+      !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1))
+    return;
+  const int place = many_before(a, b, threadIdx.x & 31);
+  if (place >= a.many || r >= ql * group) return;      // (the first kernel has reported the former)
+  float m = -INFINITY, den = 0.f, num[MERGED];
+#pragma unroll
+  for (int i = 0; i < MERGED; ++i) num[i] = 0.f;
+  const float* from = part_of(a, place, blockIdx.y, gridDim.y, kvh, 0) + threadIdx.x;
+  constexpr int STEP = (D + 2) * ROWS;      // to the next split
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, from[s * STEP + D * ROWS]);
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float ms = from[s * STEP + D * ROWS], f = ms == -INFINITY ? 0.f : fast_exp2(ms - m);
+    den = fmaf(f, from[s * STEP + (D + 1) * ROWS], den);      // (0 times a NaN is one: scores that are all none stay visible)
+#pragma unroll
+    for (int i = 0; i < MERGED; ++i) num[i] = fmaf(f, from[s * STEP + (piece * MERGED + i) * ROWS], num[i]);
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const int token = r / group, head = kvh * group + r - token * group;
+  __nv_bfloat16* dst = a.out + (size_t)(qs + token) * a.out_stride + (size_t)head * D + piece * MERGED;
+  uint32_t packed[MERGED / 2];
+#pragma unroll
+  for (int i = 0; i < MERGED / 2; ++i) packed[i] = pack_bf16(num[2 * i] * inv, num[2 * i + 1] * inv);
+  if ((((uintptr_t)dst) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < MERGED / 8; ++i)
+      reinterpret_cast<uint4*>(dst)[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+  } else {
+    const __nv_bfloat16* each = reinterpret_cast<const __nv_bfloat16*>(packed);
+#pragma unroll
+    for (int i = 0; i < MERGED; ++i) dst[i] = each[i];
+  }
+}
+
 // Keys that a request's rows reach over at most, whole tiles and one more for where the first begins.
 int span_of(int window, int most_keys, int longest) {
   const int w = window < 0 ? -window : window;
@@ -446,16 +516,22 @@ LAB_EXPORT long long lab_attention_q8_rows_scratch(int many, int n_kv, int windo
   return (long long)many * n_kv * span_of(window, most_keys, longest) * D * 4;
 }
 
+// Bytes of scratch for the splits' results of a call, none with one.
+LAB_EXPORT long long lab_attention_q8_rows_parts(int many, int n_kv, int group, int longest, int splits) {
+  return splits < 2 ? 0 : (long long)many * (((long long)longest * group + ROWS - 1) / ROWS) * n_kv * splits * (D + 2) * ROWS * 4;
+}
+
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, on 16-byte boundaries, out likewise; the `requests` from
 // request0 on, those of `fewest` rows or more (shorter ones are left alone), `many` of them, `longest` the most rows that one
-// brings; lengths are at most most_keys; scratch on a boundary of 16 bytes.  window as lab_first_key takes it.
+// brings; lengths are at most most_keys; scratch on a boundary of 16 bytes.  splits: CTAs that share the keys of a
+// tile of rows, their results in `parts` where there are several.  window as lab_first_key takes it.
 struct LabQ8Rows {
   void* out;
   const void *q, *k, *v, *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  void* scratch;
+  void *scratch, *parts;
   long long out_stride, q_stride;
-  int tokens, max_blocks, request0, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys;
+  int tokens, max_blocks, request0, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys, splits;
   float scale;
 };
 
@@ -464,6 +540,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   const int span = span_of(c->window, c->most_keys, c->longest);
   const long long rows = (long long)c->many * c->n_kv * span;
   if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->max_blocks < 1 || c->num_pages < 1 || c->fewest < 1 || c->page_size < 1 || c->request0 < 0 ||
+      c->splits < 1 || (c->splits > 1 && (c->parts == nullptr || (((uintptr_t)c->parts) & 3))) || (long long)c->n_kv * c->splits >= (1ll << 31) ||
       c->most_keys < 1 || rows >= (1ll << 31) || c->requests > 65535 || c->n_kv > 65535 || c->q_stride % 8 || (((uintptr_t)c->q) & 15) ||
       ((((uintptr_t)c->k) | ((uintptr_t)c->v) | ((uintptr_t)c->scratch)) & 15) || c->scratch == nullptr)
     return (int)cudaErrorInvalidValue;
@@ -473,7 +550,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
   a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window, a.fewest = c->fewest;
   a.tokens = c->tokens, a.request0 = c->request0, a.longest = c->longest, a.many = c->many, a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
-  a.scale_log2 = c->scale * LOG2E;
+  a.splits = c->splits, a.part = (float*)c->parts, a.scale_log2 = c->scale * LOG2E;
   CUtensorMap mk, mv;
   int rc;
   if ((rc = lab_make_map_bf16(&mk, a.wide_k, rows, D, D, KEYS))) return rc;
@@ -485,5 +562,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   if (tiles > 65535) return (int)cudaErrorInvalidValue;
   e = lab_launch(widen_kernel, dim3(span / KEYS, c->n_kv, c->requests), dim3(WIDEN_THREADS), 0, stream, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)lab_launch(attention_q8_rows_kernel, dim3(c->n_kv, (unsigned)tiles, c->requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
+  e = lab_launch(attention_q8_rows_kernel, dim3(c->n_kv * c->splits, (unsigned)tiles, c->requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
+  if (e != cudaSuccess || c->splits == 1) return (int)e;
+  return (int)lab_launch(attention_q8_rows_merge_kernel, dim3(c->n_kv * (D / MERGED), (unsigned)tiles, c->requests), dim3(ROWS), 0, stream, a);
 }

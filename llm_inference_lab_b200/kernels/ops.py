@@ -2365,7 +2365,7 @@ _pack_store = struct.Struct("9P2q9i").pack
 _pack_load = struct.Struct("7Pq5i").pack
 _pack_any = struct.Struct("10P2q10if").pack
 _pack_few = struct.Struct("11P2q13if").pack
-_pack_rows = struct.Struct("11P2q13if").pack
+_pack_rows = struct.Struct("12P2q14if").pack
 _pack_verify = struct.Struct("10P2q3i").pack
 
 
@@ -2525,6 +2525,16 @@ def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
     return 8 if 8 < splits < 16 else splits
 
 
+def q8_rows_splits(ctas: int, keys: int) -> int:
+    """CTAs that share the keys of a tile of rows in the many-rows kernel, one of them a multiprocessor at a time: as many as the GPU
+    holds, of three tiles of 128 keys at least (28 CTAs over 33 tiles: 46 us in one piece, 31 by four, 30 by five, 40 by six; 44 over
+    11: 23, by three 18, by five 23.5; 14 over 4: 13, by four 12.6, by eight 14.7), and twice as many over 128 tiles and more (34 over
+    159: 237 in one piece, 75 by four, 57 by eight; 132 over 161: 255, 190 by two; but 112 over 67: 84, 94 by two)."""
+    tiles = -(-keys // 128)
+    waves = 2 if tiles >= 128 else 1
+    return max(1, min(waves * sm_count() // max(1, ctas), tiles // 3))
+
+
 def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_len: torch.Tensor, pos0: torch.Tensor,
                  block_table: torch.Tensor, n_requests: int, q_lens, max_kv_len: int, n_q: int, n_kv: int, head_dim: int, window: int,
                  scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -2570,15 +2580,18 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)
         L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
-        L.lab_attention_q8_rows_scratch.restype = ctypes.c_longlong
+        L.lab_attention_q8_rows_scratch.restype = L.lab_attention_q8_rows_parts.restype = ctypes.c_longlong
         many = sum(1 for n in q_lens if n > few)
         each = int(L.lab_attention_q8_rows_scratch(1, n_kv, window, max_kv_len, longest))
         at_once = max(1, min(many, Q8_WIDE_BYTES // each))
+        keys = max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest)
+        splits = q8_rows_splits(n_kv * sum(-(-n * group // 128) for n in q_lens if n > few), keys)
         scratch = torch.empty((at_once * each,), dtype=_BYTE, device=q.device)
+        parts = torch.empty((int(L.lab_attention_q8_rows_parts(at_once, n_kv, group, longest, splits)),), dtype=_BYTE, device=q.device)
         for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < many else ((0, n_requests, many),):
             _check(_entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)(_pack_rows(
-                *tensors, scratch.data_ptr(), out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
-                few + 1, longest, held, max_kv_len, scale), stream), "attention_q8", 2)
+                *tensors, scratch.data_ptr(), parts.data_ptr(), out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
+                few + 1, longest, held, max_kv_len, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
     if longest_few:
         wide = q8_few_width(longest_few * group)
         if longest_few == 1 and longest == 1:

@@ -282,7 +282,11 @@ def test_a_long_portion_beside_a_single_token_takes_no_place_for_splits():
     taken = torch.cuda.max_memory_allocated() - before
     ops.take_device_errors()
     wide = n_kv * (20096 // 128 + 1) * 128 * d * 4
-    assert taken <= out.nbytes + wide + 2 * n_q * splits * (d + 2) * 4 + 2 ** 20
+    # and where the portion's keys are split too, each of its tiles of 128 rows leaves (d + 2) 32-bit numbers a row and split
+    tiles = n_kv * -(-1500 * (n_q // n_kv) // 128)
+    parts = ops.q8_rows_splits(tiles, 20001)
+    shares = tiles * parts * 128 * (d + 2) * 4 if parts > 1 else 0
+    assert taken <= out.nbytes + wide + shares + 2 * n_q * splits * (d + 2) * 4 + 2 ** 20
     alone = ops.attention_q8(x[:1], pages, args[0][:2].contiguous(), args[1][:1], args[2][:1], args[3][:1], 1, [1], 20001, n_q, n_kv, d, 0, d ** -0.5)
     assert torch.equal(out[:1], alone)
 
@@ -302,3 +306,32 @@ def test_requests_beyond_what_the_host_said_are_reported(told, rows, keys, most)
     with pytest.raises(ops.KernelError, match="row"):
         ops.take_device_errors()
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("splits", [2, 3, 7])
+@pytest.mark.parametrize("rows, past, window", [([150], [700], 0), ([150, 1, 140, 0, 300], [30, 9, 1500, 0, 0], 0), ([200], [900], 130), ([140, 160], [0, 500], -100)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_of_many_rows_in_splits(monkeypatch, splits, rows, past, window, d):
+    """More splits than some rows have tiles, and rows of which a split sees nothing; long rows also one request at a time."""
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: splits)
+    check(np.random.default_rng(17), rows, past, 4, 2, d, 16, window=window)
+    monkeypatch.setattr(ops, "Q8_WIDE_BYTES", 1)
+    check(np.random.default_rng(17), rows, past, 4, 2, d, 16, window=window)
+
+
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_rows_that_are_no_numbers_in_splits(monkeypatch, what):
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: 3)
+    got, _ = check(np.random.default_rng(18), [150], [400], 4, 2, 64, 16, change=lambda pages, batch: poison(pages, batch, 0, 480, what))
+    assert np.isnan(got).any() and not np.isnan(got).all()
+
+
+def test_rows_that_see_nothing_are_zero_in_splits(monkeypatch):
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: 2)
+    got, _ = check(np.random.default_rng(19), [150, 140], [10, 20], 4, 2, 64, 16, lengths=[0, 160])
+    assert (got[:150] == 0).all()
+
+
+def test_a_portion_behind_a_long_context_is_split():
+    assert ops.q8_rows_splits(2 * 4, 6000) > 1
+    check(np.random.default_rng(20), [140], [5860], 6, 2, 64, 64)

@@ -166,3 +166,10 @@ def test_engine_refuses_heads_that_no_kernel_takes(head_dim, taken):
     else:
         with pytest.raises(ValueError, match="heads of 272"):
             check()
+
+
+@pytest.mark.parametrize("ctas, keys, splits", [(1, 1, 1), (1, 767, 2), (1, 640, 1), (4, 4100, 11), (4, 100000, 74), (68, 20000, 4), (112, 8500, 1),
+                                                (56, 8500, 2), (132, 20600, 2), (149, 20600, 1), (500, 100000, 1), (0, 300, 1)])
+def test_splits_of_many_rows_find_room_and_keys(monkeypatch, ctas, keys, splits):
+    monkeypatch.setattr(ops, "sm_count", lambda: 148)
+    assert ops.q8_rows_splits(ctas, keys) == splits
