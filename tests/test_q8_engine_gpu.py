@@ -245,3 +245,30 @@ def test_models_that_do_not_take_it_are_refused(tmp_path_factory):
     engine = Engine(folder, "bf16", page_size=opt["page_size"], max_tokens=64, max_requests=2)
     with pytest.raises(InvalidInput, match="fixed-size state"):
         engine.verify_step([(0, 1, [2])])
+
+
+def test_drafted_steps_from_step_graphs(tmp_path_factory, monkeypatch):
+    """Steps over drafted tokens whose shape repeats are captured and replayed: the eager engine's tokens, greedy and drawn."""
+    cfg, opt = TINY["G"]
+    folder = folder_of(tmp_path_factory, "G")
+    monkeypatch.setattr(ops, "q8_few_splits", lambda *_: 1)      # (a captured step is one for a bucket of lengths)
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda *_: 1)
+    told = []
+    for graphs in (False, True):
+        rng = np.random.default_rng(6)
+        engine = Engine(folder, "bf16", page_size=opt["page_size"], max_tokens=1024, max_requests=4, cache_dtype="e4m3")
+        if graphs:
+            engine.enable_step_graphs()
+        prompts = [random_tokens(rng, n, cfg["vocab_size"]) for n in (40, 7)]
+        engine.step([Entry(r, p, [len(p) - 1]) for r, p in enumerate(prompts)])
+        held, out = [3, 5], []
+        for i in range(12):
+            drafts = [random_tokens(rng, 3, cfg["vocab_size"]) for _ in range(2)]
+            drawn = ([0.9, 0.7], [11, 12]) if i % 3 == 2 else (None, None)
+            new = engine.verify_step([(r, held[r], drafts[r]) for r in range(2)], *drawn)
+            held = [t[-1] for t in new]
+            out.append(new)
+        assert not graphs or engine.graph_replays >= 8
+        told.append((out, [engine.length(r) for r in range(2)]))
+        ops.take_device_errors()
+    assert told[0] == told[1]
