@@ -2507,8 +2507,10 @@ def _refuse_load(pages, slots, dtype):
 # Scratch of one launch over requests of many rows: those that need more go in several, one after the other (with one request at
 # least), so that many portions beside one long context do not take memory for its length each.
 Q8_WIDE_BYTES = 1 << 30
-# Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, which splits the keys.
-Q8_FEW_ROWS = 128
+# Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, by head size.  It takes 48
+# rows a CTA at most and reads the keys again for more (4 requests of 16,000 keys, few- and many-rows kernel: heads of 64, 35 rows 33
+# and 36 us, 49 rows 75 and 36; heads of 128, 84 rows 84 and 88, 112 rows 201 and 89).
+Q8_FEW_ROWS = {64: 48, 128: 96}
 
 
 def q8_few_width(rows: int) -> int:
@@ -2575,7 +2577,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             BF16 if kind is torch.bfloat16 else F32, scale), stream), "attention_q8")
         return out
     # requests of up to `few` rows, and those of more
-    few = max(1, Q8_FEW_ROWS // group) if stride % 8 == 0 and at % 16 == 0 else longest
+    few = max(1, Q8_FEW_ROWS[head_dim] // group) if stride % 8 == 0 and at % 16 == 0 else longest
     longest_few = longest
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)
