@@ -2521,7 +2521,7 @@ def q8_few_width(rows: int) -> int:
 def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
     """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once; up to eight
     merge inside their cluster, and up to sixteen are not worth a second kernel (16 requests of five drafted tokens over 1,700
-    keys: 23 us with eight, 29 with nine)."""
+    keys: 13.5 us with eight, 32 with sixteen)."""
     room = (3 if width <= 16 else 2 if width <= 32 else 1) * sm_count()
     splits = max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
     return 8 if 8 < splits < 16 else splits
@@ -2581,18 +2581,19 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     longest_few = longest
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)
-        L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
-        L.lab_attention_q8_rows_scratch.restype = L.lab_attention_q8_rows_parts.restype = ctypes.c_longlong
-        many = sum(1 for n in q_lens if n > few)
-        each = int(L.lab_attention_q8_rows_scratch(1, n_kv, window, max_kv_len, longest))
-        at_once = max(1, min(many, Q8_WIDE_BYTES // each))
+        bytes_of, parts_of = _q8_rows_bytes(head_dim)
+        many = [n for n in q_lens if n > few]
+        each = bytes_of(1, n_kv, window, max_kv_len, longest)
+        at_once = max(1, min(len(many), Q8_WIDE_BYTES // each))
         keys = max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest)
-        splits = q8_rows_splits(n_kv * sum(-(-n * group // 128) for n in q_lens if n > few), keys)
-        scratch = torch.empty((at_once * each,), dtype=_BYTE, device=q.device)
-        parts = torch.empty((int(L.lab_attention_q8_rows_parts(at_once, n_kv, group, longest, splits)),), dtype=_BYTE, device=q.device)
-        for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < many else ((0, n_requests, many),):
-            _check(_entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)(_pack_rows(
-                *tensors, scratch.data_ptr(), parts.data_ptr(), out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
+        splits = q8_rows_splits(n_kv * sum(-(-n * group // 128) for n in many), keys)
+        wide = at_once * each     # keys and values, then the splits' results (whole tiles of rows: on its boundary)
+        scratch = torch.empty((wide + (parts_of(at_once, n_kv, group, longest, splits) if splits > 1 else 0),), dtype=_BYTE, device=q.device)
+        room = scratch.data_ptr()
+        launch = _entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)
+        for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < len(many) else ((0, n_requests, len(many)),):
+            _check(launch(_pack_rows(
+                *tensors, room, room + wide, out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
                 few + 1, longest, held, max_kv_len, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
     if longest_few:
         wide = q8_few_width(longest_few * group)
@@ -2610,6 +2611,20 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             *tensors, scratch.data_ptr() if scratch is not None else 0, out.stride(0), stride, tokens, blocks, n_requests, n_q, n_kv, page_size,
             num_pages, window, few, longest_few, wide, splits, cluster, scale), stream), "attention_q8", 1 if scratch is None else 2)
     return out
+
+
+def _q8_rows_bytes(head_dim: int):
+    """The many-rows library's sizes: of the keys and values of a call, and of its splits' results."""
+    both = _q8_sizes.get(head_dim)
+    if both is None:
+        L = lib("attention_q8_rows", {"LAB_HEAD_DIM": head_dim})
+        both = _q8_sizes[head_dim] = (L.lab_attention_q8_rows_scratch, L.lab_attention_q8_rows_parts)
+        for f in both:
+            f.argtypes, f.restype = [ctypes.c_int] * 5, ctypes.c_longlong
+    return both
+
+
+_q8_sizes: dict = {}
 
 
 def _spans_of_many(q_lens, few: int, at_once: int) -> list[tuple[int, int, int]]:
