@@ -8,7 +8,11 @@
 // T = 0: accept while x_i is the argmax of its row, and end with the argmax (ties: the smallest index; a NaN never wins, and a
 // row without any number gives INT32_MAX, as the sampling kernel does).
 // The u come from the sampling kernel's hash of (seed, position, t), so a draw depends on neither the batch nor the step; u_i of
-// the test is the hash of the row's key's complement.  Probabilities are 32-bit: a test or a draw goes another way than in
+// the test is the hash of the row's key's complement.  A draft that the sampler itself drew by the request's seed was chosen by the
+// very E_t of its row: given that draft and its refusal they are no exponentials any more, and a draw by them favours what the draft
+// passed over.  A call over such drafts says so (`fresh`), and the draw after a refusal then takes a key of its own, the hash of
+// the row's.  (p = (.2, .5, .3), q = (.8, .05, .15), drafts of the sampler: (.2, .542, .258) by the row's key, p by one of its own.)
+// The draw after the last row is the sampler's in either case.  Probabilities are 32-bit: a test or a draw goes another way than in
 // exact arithmetic only where two numbers agree to about 2^-20.
 //
 // Two launches: the rows' largest entry and sum of exponentials by chunk (every logit read once: the bound, memory), then a
@@ -24,6 +28,7 @@ namespace {
 
 constexpr int CHUNK = 8192, STAT_THREADS = 256, PICK_THREADS = 512, CLUSTER = 16, KEPT = 16;
 constexpr int ROUNDS = CHUNK / (STAT_THREADS * 4);
+constexpr uint32_t FRESH = 0x3C6EF372u;      // turns a row's key into that of the draw after its refusal (any pattern would do)
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   x ^= x >> 16;
@@ -56,7 +61,7 @@ struct Args {
   const float* temperature;   // [requests], null: all 0
   const uint32_t* seeds;
   const int* positions;       // of the token that a request's first row decides
-  int rows, vocab, requests, chunks;
+  int rows, vocab, requests, chunks, fresh;
   float4* part;               // [rows, chunks]: largest entry, sum of exponentials relative to it, its index
   int *tokens, *counts;
 };
@@ -219,9 +224,9 @@ __global__ void __launch_bounds__(PICK_THREADS, 2) verify_pick_kernel(const Args
   Best best = {0.f, 0.f, INT_MAX, INT_MAX};      // a weight above 0 is wanted
   if (!greedy && n > 0) {
     const float m = ends.x, inverse_sum = 1.f / ends.y;
-    const uint32_t key = key_of(stop);
-    const float* lr = a.logits + (size_t)row * a.ld;
     const bool over = stop == n - 1;
+    const uint32_t key = a.fresh && !over ? mix32(key_of(stop) ^ FRESH) : key_of(stop);
+    const float* lr = a.logits + (size_t)row * a.ld;
     const float* qr = !over && a.draft_probs != nullptr ? a.draft_probs + (size_t)row * a.ld_probs : nullptr;
     const int certain = !over && a.draft_probs == nullptr ? a.drafts[row] : -1;
     // w / E <= w / (1 - u), so most entries are passed over without a logarithm: those that cannot beat what the warp has found.
@@ -316,8 +321,8 @@ LAB_EXPORT int lab_verify_chunk() { return CHUNK; }
 
 // A call, as the host packs it.  logits [rows, vocab] 32-bit, rows `ld` apart; draft_probs likewise or null; drafts [rows]: the token
 // drafted after a row's (a request's last row has none); starts [requests + 1]; temperature, seeds, positions [requests], null:
-// greedy.  tokens [rows]: what a request's rows give, drafts that were accepted, the token that ends it, -1 behind it; counts
-// [requests].
+// greedy; fresh: the draw after a refusal takes random numbers of its own.  tokens [rows]: what a request's rows give, drafts that
+// were accepted, the token that ends it, -1 behind it; counts [requests].
 struct LabVerify {
   int *tokens, *counts;
   const float *logits, *draft_probs;
@@ -327,7 +332,7 @@ struct LabVerify {
   const int* positions;
   void* scratch;
   long long ld, ld_probs;
-  int rows, vocab, requests;
+  int rows, vocab, requests, fresh;
 };
 
 LAB_EXPORT int lab_verify_drafts(const LabVerify* c, cudaStream_t stream) {
@@ -341,7 +346,7 @@ LAB_EXPORT int lab_verify_drafts(const LabVerify* c, cudaStream_t stream) {
   Args a;
   a.logits = c->logits, a.ld = c->ld, a.draft_probs = c->draft_probs, a.ld_probs = c->ld_probs, a.drafts = c->drafts, a.starts = c->starts;
   a.temperature = temperature, a.seeds = c->seeds, a.positions = c->positions;
-  a.rows = rows, a.vocab = vocab, a.requests = requests, a.chunks = (vocab + CHUNK - 1) / CHUNK;
+  a.rows = rows, a.vocab = vocab, a.requests = requests, a.fresh = c->fresh, a.chunks = (vocab + CHUNK - 1) / CHUNK;
   a.part = (float4*)scratch, a.tokens = c->tokens, a.counts = c->counts;
   if (rows > 0) {
     const cudaError_t e = lab_launch(temperature != nullptr ? verify_chunks_kernel<true> : verify_chunks_kernel<false>, dim3(a.chunks, rows), dim3(STAT_THREADS), 0, stream, a);

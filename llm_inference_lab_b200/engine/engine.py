@@ -250,7 +250,8 @@ class Engine:
         refused leaves the cache again.  Returns each request's new tokens: the accepted drafts, and one drawn behind them, which
         is not in the cache yet and is the token to go on with.
 
-        `temperatures` and `seeds` one per request (None: greedy); a token's draw goes by its position, as everywhere, so with
+        `temperatures` and `seeds` one per request (None: greedy); a token's draw goes by its position, as everywhere, and what
+        replaces a refused draft by random numbers of its own, so that the drafts may come from an engine with the same seeds: with
         or without drafts a seed gives tokens of the same distribution (greedy: the same tokens).  `draft_probs`: for every
         row of the step, in order, the probabilities that its draft was drawn from, [rows, vocab] 32-bit (a request's last row:
         anything); None: the drafts are certain.  Models with fixed-size state are refused: it cannot go back."""
@@ -276,7 +277,7 @@ class Engine:
                 ints = torch.tensor([*(int(s) & 0x7FFFFFFF for s in seeds), *held], dtype=torch.int32).to(self.device, non_blocking=True)
                 drawn = [torch.tensor(list(temperatures), dtype=torch.float32).to(self.device, non_blocking=True), ints[: len(pairs)],
                          ints[len(pairs):]]
-            tokens, counts = ops.verify_drafts(logits, meta[: len(flat)], meta[len(flat):], draft_probs, *drawn)
+            tokens, counts = ops.verify_drafts(logits, meta[: len(flat)], meta[len(flat):], draft_probs, *drawn, fresh=True)
             told = torch.cat((tokens, counts)).cpu().tolist()
             new = [told[at: at + n] for at, n in zip(starts, told[len(flat):])]
             for picked in new:

@@ -2366,7 +2366,7 @@ _pack_load = struct.Struct("7Pq5i").pack
 _pack_any = struct.Struct("10P2q10if").pack
 _pack_few = struct.Struct("11P2q13if").pack
 _pack_rows = struct.Struct("12P2q14if").pack
-_pack_verify = struct.Struct("10P2q3i").pack
+_pack_verify = struct.Struct("10P2q4i").pack
 
 
 _entries: dict = {}    # (library, entry, head size) -> the entry, which takes a record and a stream
@@ -2665,14 +2665,20 @@ _verify_chunk = 0     # entries of a row that a block of the first kernel takes,
 
 
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tensor, draft_probs: torch.Tensor | None = None,
-                  temperature: torch.Tensor | None = None, seeds: torch.Tensor | None = None, positions: torch.Tensor | None = None):
+                  temperature: torch.Tensor | None = None, seeds: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                  fresh: bool = False):
     """Judges drafted tokens by the target's 32-bit logits [rows, vocab] and draws the token that follows the accepted ones.
 
     Request b's rows are starts[b] .. starts[b + 1] (int32 [requests + 1], ascending): one after the token it holds, one after
     each drafted token.  drafts [rows] int32: the token drafted after a row's; a request's last row has none, whatever stands
     there.  `draft_probs` [rows, vocab] 32-bit: the probabilities each draft was drawn from (None: drafts are certain, as an
     argmax or a copied n-gram is); `temperature`, `seeds`, `positions` per request as `sample` takes them, positions that of the
-    token a request's first row decides; no temperature, or 0: greedy.  Emitted tokens are distributed as the target's own.
+    token a request's first row decides; no temperature, or 0: greedy.
+
+    Emitted tokens are distributed as the target's own where the drafts do not depend on the random numbers that replace them.
+    Those are `sample`'s for (seed, position), so drafts that `sample` or an engine drew need either other seeds than these or
+    `fresh`: the draw after a refusal then takes numbers that no other draw has.  (The draw behind the last draft, and that of a
+    request without drafts, is `sample`'s own in either case.)
 
     Returns (tokens [rows], counts [requests]), int32: counts[b] tokens from row starts[b] on, drafts that were accepted and then
     the drawn one, -1 behind them; rows of no request hold nothing.  A row without any number gives INT32_MAX, as `sample` does."""
@@ -2700,7 +2706,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, starts: torch.Tens
         at + 4 * behind, at + 4 * (behind + rows), logits.data_ptr(), draft_probs.data_ptr() if draft_probs is not None else 0,
         drafts.data_ptr(), starts.data_ptr(), temperature.data_ptr() if drawn else 0, seeds.data_ptr() if drawn else 0,
         positions.data_ptr() if drawn else 0, at, logits.stride(0), draft_probs.stride(0) if draft_probs is not None else 0, rows, vocab,
-        requests), _current(device)), "verify_drafts", 2 if rows else 1)
+        requests, bool(fresh)), _current(device)), "verify_drafts", 2 if rows else 1)
     return tokens, counts
 
 
