@@ -13,7 +13,8 @@
 // addend of the exponent: p' = 2^(s + e_v - M) with M the largest exponent of the TILE, per row.  A tile's p' then reach from
 // 256 down to 2^-10, whatever earlier tiles held, so that a long tail behind one dominant key keeps its weight; the tile's O^T is
 // read from tensor memory and added to the sums in registers with 2^(M - R), R the running reference.  A tile's sum of p
-// without e_v is kept a thread for its own keys, and added over the threads once at the end.
+// without e_v is kept a thread for its own keys, and added over the threads once at the end.  (It is p' 2^-e_v: where a
+// tile's values are rows of scales up to 2^90 apart and below 2^80, every weight down to 2^-44 of the largest is in it.)
 //
 // Warp 0 loads (TMA, a page a lane), warp 1 issues the products and owns tensor memory, warps 2-5 (128 threads) do the rest.
 // The scores of tile j + 1 are formed beside the softmax of tile j, and O^T of tile j - 1 beside it too.  The keys are split
@@ -355,14 +356,21 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
       }
       if (__any_sync(0xffffffffu, unit)) {
         // A scale of one may be that of a value of zeros, which must not set the tile's largest p' (behind a first token with
-        // all the weight and nothing to say the others' p' would be below the smallest code): it takes the least scale instead.
+        // all the weight and nothing to say the others' p' would be below the smallest code).  Any other power gives the same
+        // sums: it takes one 2^60 below the largest of the warp's other values, so that a key of 2^60 times the others' weight
+        // leaves them theirs, and that its own weight reaches the sum down to 2^-60 of the largest.
         ok &= __all_sync(0xffffffffu, mbar_wait(&bar->v_full[j % STAGES], (j / STAGES) & 1, abort_flag));
+        uint32_t any = unit ? 0u : 1u;
         if (unit) {
           const uint4* z = reinterpret_cast<const uint4*>(smem + L::OFF_V + (j % STAGES) * Tile::BYTES + mine * D);
-          uint32_t any = 0;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) any |= z[c].x | z[c].y | z[c].z | z[c].w;
-          if ((any & 0x7f7f7f7fu) == 0) vexp = Q8_LEAST_POWER, v_inv = __uint_as_float((uint32_t)(127 - Q8_LEAST_POWER) << 23) * FROM_CODES;
+        }
+        const bool nothing = (any & 0x7f7f7f7fu) == 0;
+        const float others = warp_max_number(held && !nothing && vexp < 128.f ? vexp : -INFINITY);      // (128: a value that is no number)
+        if (nothing) {
+          vexp = fmaxf((others == -INFINITY ? 0.f : others) - 60.f, (float)Q8_LEAST_POWER);
+          v_inv = __uint_as_float((uint32_t)(127 - (int)vexp) << 23) * FROM_CODES;
         }
       }
       const int sb = j & 1;

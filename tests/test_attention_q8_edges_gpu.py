@@ -1,0 +1,56 @@
+"""Attention over the 8-bit cache where values are nothing, batches are mixed, host and device disagree, and scratch is scarce."""
+import numpy as np
+import pytest
+import torch
+
+from llm_inference_lab_b200.kernels import ops
+from q8_helpers import Batch, attention, random_pages
+from test_attention_q8_gpu import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("e", [0, 10, 20, 30])
+@pytest.mark.parametrize("rows, past", [([1], [3000]), ([5], [3000]), ([140], [2000])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_whose_values_are_nothing_keep_their_weight(rows, past, d, e):
+    """Most values are rows of zeros, every 61st is of scale 2^e: the zeros' keys belong to the softmax's sum all the same."""
+    rng = np.random.default_rng(21)
+
+    def values(pages, batch):
+        keep = torch.zeros(tuple(pages.v_scale.shape), dtype=torch.bool, device="cuda")
+        for j in range(0, batch.held[0], 61):
+            keep[int(batch.table[0, j // batch.page_size]), :, j % batch.page_size] = True
+        pages.v.view(torch.uint8)[~keep] = 0
+        pages.v_scale[~keep] = 127
+        pages.v_scale[keep] = 127 + e
+    check(rng, rows, past, 4, 2, d, 16, change=values, tail=0)
+
+
+@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("splits", [1, 4, 20])
+def test_tiles_of_nothing_keep_their_weight(monkeypatch, rows, splits):
+    """Whole tiles of keys whose values are zeros, 2^-18 of the largest weight each and thousands of them: 1.5 % of the sum."""
+    monkeypatch.setattr(ops, "q8_few_splits", lambda *_: splits)
+    rng = np.random.default_rng(22)
+    d, n_q, page, past = 64, 2, 16, 4090
+    batch = Batch(rng, [rows], [past], page)
+    pages = random_pages(ops, rng, batch.num_pages, 1, page, d, spread=0.0)
+    first = batch.table[0, : 4096 // page].astype(np.int64)[: -8]      # all but the last tile
+    pages.k[:] = 0.0
+    pages.k_scale[:] = 127
+    pages.v.view(torch.uint8)[first] = 0
+    pages.v_scale[first] = 127
+    pages.v_scale[batch.table[0, 4096 // page - 8:].astype(np.int64)] = 131
+    last = batch.table[0, 4096 // page - 8].astype(np.int64)
+    pages.k[last, 0, 0, 0] = 1.0                                       # one key of the last tile has nearly all the weight
+    q = np.zeros((rows, n_q * d))
+    q[:, ::d] = 12.5 * d ** 0.5                                        # e^12.5 = 2^18.03
+    x = torch.from_numpy(q.astype(np.float32)).cuda().to(torch.bfloat16)
+    out = ops.attention_q8(x, pages, *batch.args(), n_q, 1, d, 0, d ** -0.5).double().cpu().numpy()
+    ops.take_device_errors()
+    want, bound = attention(x, pages, batch, n_q, 1, d, 0, d ** -0.5, True)
+    assert (np.abs(out - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all()
+    # the values of the last tile as if the others' keys were not there: 1.5 % off, and farther than what is allowed
+    away = np.abs(want) * 0.014 > bound + 2.0 ** -8 * (np.abs(want) + bound)
+    assert away.any()
