@@ -2581,11 +2581,12 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     longest_few = longest
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)
+        most_keys = max(1, max_kv_len)      # (rows that see nothing are still written)
         bytes_of, parts_of = _q8_rows_bytes(head_dim)
         many = [n for n in q_lens if n > few]
-        each = bytes_of(1, n_kv, window, max_kv_len, longest)
+        each = bytes_of(1, n_kv, window, most_keys, longest)
         at_once = max(1, min(len(many), Q8_WIDE_BYTES // each))
-        keys = max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest)
+        keys = most_keys if window == 0 else min(most_keys, abs(window) + longest)
         splits = q8_rows_splits(n_kv * sum(-(-n * group // 128) for n in many), keys)
         wide = at_once * each     # keys and values, then the splits' results (whole tiles of rows: on its boundary)
         scratch = torch.empty((wide + (parts_of(at_once, n_kv, group, longest, splits) if splits > 1 else 0),), dtype=_BYTE, device=q.device)
@@ -2594,7 +2595,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < len(many) else ((0, n_requests, len(many)),):
             _check(launch(_pack_rows(
                 *tensors, room, room + wide, out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
-                few + 1, longest, held, max_kv_len, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
+                few + 1, longest, held, most_keys, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
     if longest_few:
         wide = q8_few_width(longest_few * group)
         if longest_few == 1 and longest == 1:

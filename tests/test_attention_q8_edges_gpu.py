@@ -54,3 +54,13 @@ def test_tiles_of_nothing_keep_their_weight(monkeypatch, rows, splits):
     # the values of the last tile as if the others' keys were not there: 1.5 % off, and farther than what is allowed
     away = np.abs(want) * 0.014 > bound + 2.0 ** -8 * (np.abs(want) + bound)
     assert away.any()
+
+
+def test_long_portions_that_see_no_key_at_all():
+    """Every request's length is nothing: zeros, whatever the kernel."""
+    batch = Batch(np.random.default_rng(23), [150, 1, 130], [0, 0, 0], 16, lengths=[0, 0, 0])
+    pages = random_pages(ops, np.random.default_rng(23), 2, 2, 16, 64)
+    x = torch.ones((batch.tokens, 4 * 64), dtype=torch.bfloat16, device="cuda")
+    out = ops.attention_q8(x, pages, *batch.args(), 4, 2, 64, 0, 0.125, out=torch.full_like(x, 7.0))
+    ops.take_device_errors()
+    assert (out == 0).all()
