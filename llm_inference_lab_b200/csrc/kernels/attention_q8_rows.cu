@@ -191,14 +191,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   const int b = a.request0 + blockIdx.z, split = blockIdx.x / a.n_kv, kvh = blockIdx.x - split * a.n_kv, group = a.n_q / a.n_kv;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
-  const int p0 = a.pos0[b];
-  if (ql < a.fewest || r0 >= ql * group || !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) {
+  const int p0 = a.pos0[b], lane = threadIdx.x & 31;
+  // (a request that the host has not counted has no place in scratch: the first kernel reports it, and its rows stay as they are)
+  if (ql < a.fewest || r0 >= ql * group || many_before(a, b, lane) >= a.many ||
+      !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) {
     pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
     return;
   }
   // The warp's number from one lane, so that the compiler sees a warp's branches as its lanes' common ones: for heads of 128 alone (two
   // portions of 1,024 rows: 134.7 us, 140.4 without; heads of 64: 74.9 and 70.7, 8,192 rows 178 and 165).
-  const int warp = D == 128 ? __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0) : (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int warp = D == 128 ? __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0) : (int)(threadIdx.x >> 5);
   const int last_row = min(r0 + ROWS, ql * group) - 1;
   const int pos_lo = p0 + r0 / group, pos_hi = p0 + last_row / group;
   const int last = min(min(pos_hi, a.kv_len[b] - 1), a.max_blocks * a.page_size - 1), first = lab_first_key(pos_lo, a.window);
@@ -413,9 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     }
     if (ok && a.splits > 1) {      // half of the head's entries a group, neighbouring rows side by side
       tc_fence_after();
-      const int place = many_before(a, b, lane);
-      const bool room = place < a.many;      // (more of them than the host counted: the first kernel has reported it)
-      float* to = part_of(a, room ? place : 0, gridDim.y - 1 - blockIdx.y, gridDim.y, kvh, split) + mine;
+      float* to = part_of(a, many_before(a, b, lane), gridDim.y - 1 - blockIdx.y, gridDim.y, kvh, split) + mine;
 #pragma unroll
       for (int part = 0; part < D / 64; ++part) {
         uint32_t x[32];
@@ -423,9 +423,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
         tmem_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (room) to[(g * (D / 2) + part * 32 + i) * ROWS] = n_tiles == 0 ? 0.f : __uint_as_float(x[i]);
+          to[(g * (D / 2) + part * 32 + i) * ROWS] = n_tiles == 0 ? 0.f : __uint_as_float(x[i]);
       }
-      if (g == 0 && room) to[D * ROWS] = n_tiles == 0 ? -INFINITY : *reference, to[(D + 1) * ROWS] = l;
+      if (g == 0) to[D * ROWS] = n_tiles == 0 ? -INFINITY : *reference, to[(D + 1) * ROWS] = l;
     } else if (ok) {      // half of the head's entries a group
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -64,3 +64,21 @@ def test_long_portions_that_see_no_key_at_all():
     out = ops.attention_q8(x, pages, *batch.args(), 4, 2, 64, 0, 0.125, out=torch.full_like(x, 7.0))
     ops.take_device_errors()
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_portion_that_the_host_has_not_counted_is_left_alone(monkeypatch, splits, d):
+    """Told one portion of 200 rows and a single token, the device has two of 200: the second is reported and its rows stay."""
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: splits)
+    rng = np.random.default_rng(25)
+    batch = Batch(rng, [200, 200], [30, 40], 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, d)
+    q_start, kv_len, pos0, table, *_ = batch.args()
+    q = torch.from_numpy(rng.standard_normal((400, 4 * d)).astype(np.float32)).cuda().to(torch.bfloat16)
+    want = ops.attention_q8(q, pages, q_start, kv_len, pos0, table, 2, [200, 200], 240, 4, 2, d, 0, d ** -0.5)
+    out = torch.full_like(q, 7.0)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, 2, [200, 1], 240, 4, 2, d, 0, d ** -0.5, out=out)
+    with pytest.raises(ops.KernelError, match="row"):
+        ops.take_device_errors()
+    assert torch.equal(out[:200], want[:200]) and (out[200:] == 7.0).all()
