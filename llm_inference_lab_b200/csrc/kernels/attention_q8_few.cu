@@ -71,7 +71,7 @@ struct Args {
   long long q_stride;
   const uint8_t *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  int tokens, max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, longest, splits, cluster;
+  int tokens, max_blocks, n_q, n_kv, page_size, num_pages, window, most_rows, longest, splits, cluster, alone;
   bool by_request;      // the splits' results: `longest` places a request, else one a row of the batch
   float scale_log2;
   float *part_acc, *part_ml;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(THREADS, N <= 16 ? 3 : N <= 32 ? 2 : 1) attent
   const int r0 = (blockIdx.y - kvh * tiles_of_rows) * N;       // first row: row r is token r / group, head r % group
   const bool within = qs >= 0 && qs <= a.tokens - ql && ql <= a.longest;      // what the host has been told
   if (ql > a.most_rows || r0 >= ql * group || !within) {
-    if (ql <= a.most_rows && !within && r0 == 0 && threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
+    if ((ql <= a.most_rows || a.alone) && !within && r0 == 0 && threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
     pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
     return;
   }
@@ -646,9 +646,9 @@ int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, dim3
 }  // namespace
 
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise; requests of up to most_rows rows (longer
-// ones are left alone), `longest` the most that one of them brings; width: rows a CTA takes, 16, 32 or 48; splits of the keys, merged
-// inside their cluster (`cluster`, up to eight) or by a second kernel through scratch: n_q * splits * (D + 2)
-// floats for each of min(tokens, requests * longest) rows.
+// ones are left alone, and reported where no other call takes them: `alone`), `longest` the most that one of them brings; width: rows a
+// CTA takes, 16, 32 or 48; splits of the keys, merged inside their cluster (`cluster`, up to eight) or by a second kernel through
+// scratch: n_q * splits * (D + 2) floats for each of min(tokens, requests * longest) rows.
 // window as lab_first_key takes it.
 struct LabQ8Few {
   void* out;
@@ -656,7 +656,7 @@ struct LabQ8Few {
   const int *q_start, *kv_len, *pos0, *block_table;
   float* scratch;
   long long out_stride, q_stride;
-  int tokens, max_blocks, requests, n_q, n_kv, page_size, num_pages, window, most_rows, longest, width, splits, cluster;
+  int tokens, max_blocks, requests, n_q, n_kv, page_size, num_pages, window, most_rows, longest, width, splits, cluster, alone;
   float scale;
 };
 
@@ -677,7 +677,7 @@ LAB_EXPORT int lab_attention_q8_few(const LabQ8Few* c, cudaStream_t stream) {
   a.k_scale = (const uint8_t*)c->k_scale, a.v_scale = (const uint8_t*)c->v_scale;
   a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
   a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window;
-  a.most_rows = c->most_rows, a.splits = c->splits, a.cluster = c->cluster, a.scale_log2 = c->scale * LOG2E;
+  a.most_rows = c->most_rows, a.splits = c->splits, a.cluster = c->cluster, a.alone = c->alone, a.scale_log2 = c->scale * LOG2E;
   const bool second = c->splits > 1 && !c->cluster;
   a.tokens = c->tokens, a.longest = c->longest;
   const long long places = (long long)c->requests * c->longest;

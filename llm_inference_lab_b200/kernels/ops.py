@@ -2364,7 +2364,7 @@ _device_now = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") e
 _pack_store = struct.Struct("9P2q9i").pack
 _pack_load = struct.Struct("7Pq5i").pack
 _pack_any = struct.Struct("10P2q10if").pack
-_pack_few = struct.Struct("11P2q13if").pack
+_pack_few = struct.Struct("11P2q14if").pack
 _pack_rows = struct.Struct("12P2q14if").pack
 _pack_verify = struct.Struct("10P2q4i").pack
 
@@ -2549,7 +2549,8 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `Q8_FEW_ROWS` rows
     and query heads of a kv head take scratch for their keys and values in bfloat16, `max_kv_len` of them or what a window leaves,
     up to `Q8_WIDE_BYTES` at a time.  A request beyond `q_lens`, the rows of q or `max_kv_len` is reported (`take_device_errors`)
-    where a kernel's work is sized by them, and its rows stay as they are."""
+    where a kernel's work is sized by them, and its rows stay as they are; so is one that by its own rows belongs to the kernel for
+    few of them and has more than any that `q_lens` gives that kernel."""
     k, v, ks, vs = pages
     device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
     shape = q.shape
@@ -2582,6 +2583,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)
         most_keys = max(1, max_kv_len)      # (rows that see nothing are still written)
+        fewest = few + 1 if longest_few else 1      # (with no call for the others, a request that turns out shorter belongs here too)
         bytes_of, parts_of = _q8_rows_bytes(head_dim)
         many = [n for n in q_lens if n > few]
         each = bytes_of(1, n_kv, window, most_keys, longest)
@@ -2595,7 +2597,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < len(many) else ((0, n_requests, len(many)),):
             _check(launch(_pack_rows(
                 *tensors, room, room + wide, out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
-                few + 1, longest, held, most_keys, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
+                fewest, longest, held, most_keys, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
     if longest_few:
         wide = q8_few_width(longest_few * group)
         if longest_few == 1 and longest == 1:
@@ -2610,7 +2612,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             scratch = torch.empty((places * n_q * splits * (head_dim + 2),), dtype=torch.float32, device=q.device)
         _check(_entry("attention_q8_few", "lab_attention_q8_few", head_dim)(_pack_few(
             *tensors, scratch.data_ptr() if scratch is not None else 0, out.stride(0), stride, tokens, blocks, n_requests, n_q, n_kv, page_size,
-            num_pages, window, few, longest_few, wide, splits, cluster, scale), stream), "attention_q8", 1 if scratch is None else 2)
+            num_pages, window, few, longest_few, wide, splits, cluster, longest <= few, scale), stream), "attention_q8", 1 if scratch is None else 2)
     return out
 
 

@@ -82,3 +82,37 @@ def test_a_portion_that_the_host_has_not_counted_is_left_alone(monkeypatch, spli
     with pytest.raises(ops.KernelError, match="row"):
         ops.take_device_errors()
     assert torch.equal(out[:200], want[:200]) and (out[200:] == 7.0).all()
+
+
+@pytest.mark.parametrize("told, rows", [([1, 1], [1, 130]), ([5, 5, 5], [5, 60, 5]), ([1], [400])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_request_longer_than_any_that_was_told_is_reported(told, rows, d):
+    """The host's counts need the kernel for few rows alone; on the device one request has more than that kernel takes."""
+    rng = np.random.default_rng(26)
+    batch = Batch(rng, rows, [9] * len(rows), 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, d)
+    q_start, kv_len, pos0, table, *_ = batch.args()
+    q = torch.ones((batch.tokens, 4 * d), dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, torch.nan)      # (no result of these inputs is one)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, len(told), told, 500, 4, 2, d, 0, d ** -0.5, out=out)
+    with pytest.raises(ops.KernelError, match="row"):
+        ops.take_device_errors()
+    b = rows.index(max(rows))
+    untouched = torch.isnan(out)
+    own = slice(batch.starts[b], batch.starts[b + 1])
+    assert untouched[own].all() and int(untouched.sum()) == untouched[own].numel()
+
+
+@pytest.mark.parametrize("told, rows", [([200], [1]), ([150, 200], [3, 160]), ([200, 0], [0, 2]), ([200, 1], [130, 1])])
+def test_requests_shorter_than_told_are_attended(told, rows):
+    rng = np.random.default_rng(27)
+    batch = Batch(rng, rows, [70] * len(rows), 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 64)
+    q_start, kv_len, pos0, table, _, _, most = batch.args()
+    q = torch.from_numpy(rng.standard_normal((sum(told), 4 * 64)).astype(np.float32)).cuda().to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, len(told), told, most, 4, 2, 64, 0, 0.125, out=out)
+    ops.take_device_errors()
+    got = out[: batch.tokens].double().cpu().numpy()
+    want, bound = attention(q[: batch.tokens], pages, batch, 4, 2, 64, 0, 0.125, True)
+    assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all() and (out[batch.tokens:] == 7.0).all()
