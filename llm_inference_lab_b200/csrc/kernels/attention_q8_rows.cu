@@ -74,7 +74,7 @@ struct Args {
   long long q_stride;
   const uint8_t *k, *v, *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
-  int tokens, max_blocks, request0, n_q, n_kv, page_size, num_pages, window, fewest, longest, many;
+  int tokens, max_blocks, request0, requests, look0, look1, n_q, n_kv, page_size, num_pages, window, fewest, longest, many;
   __nv_bfloat16 *wide_k, *wide_v;      // [requests of many rows][n_kv][span][D]
   int span;                            // keys, a multiple of KEYS
   int splits;                          // of the keys of a tile of rows
@@ -84,8 +84,32 @@ struct Args {
 
 // A request's keys in scratch start at the tile of the first that its rows see.
 __device__ __forceinline__ int first_tile(int pos0, int window) { return lab_first_key(pos0, window) / KEYS; }
-// The request's number among the launch's of many rows: by one warp, all its lanes get it.
-__device__ __forceinline__ int many_before(const Args& a, int b, int lane) {
+// The grids have a slice (z) for each of the `many` requests of many rows that the host has counted, not for every request: beside one
+// portion 63 single tokens made 63 slices of CTAs that found nothing to do (a portion of 2,048 rows, 14 + 2 heads of 64: 120 us with the
+// few-rows kernel's 11, 42 now; 28 + 4 heads of 128: 264 with 37, 117 now).  Slice z belongs to the z-th of them, -1 where the device's
+// counts have no such; by one warp, all its lanes get it.  Where all requests of a run have many rows (MIXED false) no lookup is
+// needed: builds of their own, since a lookup's loads and code cost about 1 us (2,048 rows beside one token: 40.1 us, 38.9 without; two
+// portions of 1,024 rows of 28 + 4 heads 137.8, 137.3).
+template <bool MIXED> __device__ __forceinline__ int request_of(const Args& a, int z, int lane) {
+  if constexpr (MIXED) {
+    int left = z;
+    for (int i0 = 0; i0 < a.requests; i0 += 32) {
+      const int i = a.request0 + i0 + lane;
+      const uint32_t found = __ballot_sync(0xffffffffu, i0 + lane < a.requests && a.q_start[i + 1] - a.q_start[i] >= a.fewest);
+      const int here = __popc(found);
+      if (left < here) return a.request0 + i0 + (int)__fns(found, 0, left + 1);
+      left -= here;
+    }
+    return -1;
+  } else {
+    return a.request0 + z;
+  }
+}
+
+// The place of a request's keys and values in scratch: its number among those of many rows.  (Also where that is the slice's as a rule: so
+// the attention's loop keeps the registers it had, 8,192 rows of 14 + 2 heads of 64 in 193 us, 200 with z itself.)
+template <bool MIXED> __device__ __forceinline__ int place_of(const Args& a, int b, int z, int lane) {
+  if constexpr (MIXED) return z;
   int n = 0;
   for (int i = a.request0 + lane; i < b; i += 32) n += a.q_start[i + 1] - a.q_start[i] >= a.fewest;
   return __reduce_add_sync(0xffffffffu, n);
@@ -105,10 +129,24 @@ __device__ __forceinline__ float* part_of(const Args& a, int place, int tile, in
 // Codes to bfloat16: a CTA a tile of keys of one request and kv head, 16 codes of a key and 16 of a value a thread and turn.
 // ----------------------------------------------------------------------------------------
 constexpr int WIDEN_THREADS = 256;
+template <bool MIXED>
 __global__ void __launch_bounds__(WIDEN_THREADS) widen_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
-  const int b = a.request0 + blockIdx.z, kvh = blockIdx.y;
+  const int kvh = blockIdx.y, lane = threadIdx.x & 31;
+  // Requests of many rows for which there is no slice, from look0 up to look1: one warp of the launch looks for such.
+  if (blockIdx.x == 0 && kvh == 0 && blockIdx.z == 0 && threadIdx.x >= WIDEN_THREADS - 32) {
+    int left = a.many;      // of the slices
+    for (int i = a.look0 + lane; i - lane < a.look1; i += 32) {
+      const bool many = i < a.look1 && a.q_start[i + 1] - a.q_start[i] >= a.fewest, inside = i >= a.request0 && i < a.request0 + a.requests;
+      left -= __popc(__ballot_sync(0xffffffffu, many && inside));
+      if (__any_sync(0xffffffffu, many && !inside)) left = -1;
+      if (left < 0) break;
+    }
+    if (left < 0 && lane == 0) lab_set_error(LAB_ERR_ROW_RANGE);
+  }
+  const int b = request_of<MIXED>(a, blockIdx.z, lane);
+  if (MIXED && b < 0) return;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   if (ql < a.fewest) return;
   const int p0 = a.pos0[b], first = lab_first_key(p0, a.window);
@@ -120,12 +158,7 @@ __global__ void __launch_bounds__(WIDEN_THREADS) widen_kernel(const Args a) {
   }
   if (key0 > last) return;
   const int* bt = a.block_table + (size_t)b * a.max_blocks;
-  const int place = many_before(a, b, threadIdx.x & 31);
-  if (place >= a.many) {      // more of them than the host counted: scratch has no room
-    if (threadIdx.x == 0) lab_set_error(LAB_ERR_ROW_RANGE);
-    return;
-  }
-  const size_t to0 = (((size_t)place * a.n_kv + kvh) * a.span + (size_t)blockIdx.x * KEYS) * D;
+  const size_t to0 = (((size_t)place_of<MIXED>(a, b, blockIdx.z, lane) * a.n_kv + kvh) * a.span + (size_t)blockIdx.x * KEYS) * D;
   constexpr int PIECES = D / 16, TURNS = KEYS * PIECES / WIDEN_THREADS;
   static_assert(KEYS * PIECES % WIDEN_THREADS == 0, "whole turns");
   uint4 kc[TURNS], vc[TURNS];
@@ -179,6 +212,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
+template <bool MIXED>
 __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                        const __grid_constant__ CUtensorMap map_v, const Args a) {
   extern __shared__ uint8_t smem_raw[];
@@ -188,19 +222,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
   pdl_trigger();
   // Until pdl_wait() below only the step's metadata is read (no kernel of the step writes it).
   // kv heads fastest, a request's last rows first: the CTAs that walk the most keys start in the first wave
-  const int b = a.request0 + blockIdx.z, split = blockIdx.x / a.n_kv, kvh = blockIdx.x - split * a.n_kv, group = a.n_q / a.n_kv;
+  const int split = blockIdx.x / a.n_kv, kvh = blockIdx.x - split * a.n_kv, group = a.n_q / a.n_kv;
+  const int b = request_of<MIXED>(a, blockIdx.z, threadIdx.x & 31);
+  if (MIXED && b < 0) {
+    pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
+    return;
+  }
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
-  const int p0 = a.pos0[b], lane = threadIdx.x & 31;
-  // (a request that the host has not counted has no place in scratch: the first kernel reports it, and its rows stay as they are)
-  if (ql < a.fewest || r0 >= ql * group || many_before(a, b, lane) >= a.many ||
-      !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) {
-    pdl_wait();  // this kernel ends only after the one before it: what follows may count on both
+  const int p0 = a.pos0[b];
+  if (ql < a.fewest || r0 >= ql * group || !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) {
+    pdl_wait();
     return;
   }
   // The warp's number from one lane, so that the compiler sees a warp's branches as its lanes' common ones: for heads of 128 alone (two
   // portions of 1,024 rows: 134.7 us, 140.4 without; heads of 64: 74.9 and 70.7, 8,192 rows 178 and 165).
-  const int warp = D == 128 ? __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0) : (int)(threadIdx.x >> 5);
+  const int warp = D == 128 ? __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0) : (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int last_row = min(r0 + ROWS, ql * group) - 1;
   const int pos_lo = p0 + r0 / group, pos_hi = p0 + last_row / group;
   const int last = min(min(pos_hi, a.kv_len[b] - 1), a.max_blocks * a.page_size - 1), first = lab_first_key(pos_lo, a.window);
@@ -236,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ---------------- loader ----------------
-      const int row0 = (many_before(a, b, lane) * a.n_kv + kvh) * a.span + (t_lo - first_tile(p0, a.window)) * KEYS;
+      const int row0 = (place_of<MIXED>(a, b, blockIdx.z, lane) * a.n_kv + kvh) * a.span + (t_lo - first_tile(p0, a.window)) * KEYS;
       if (lane == 0) {
         int asked = 0;
         for (int j = 0; j < n_tiles; ++j) {
@@ -415,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
     }
     if (ok && a.splits > 1) {      // half of the head's entries a group, neighbouring rows side by side
       tc_fence_after();
-      float* to = part_of(a, many_before(a, b, lane), gridDim.y - 1 - blockIdx.y, gridDim.y, kvh, split) + mine;
+      float* to = part_of(a, blockIdx.z, gridDim.y - 1 - blockIdx.y, gridDim.y, kvh, split) + mine;
 #pragma unroll
       for (int part = 0; part < D / 64; ++part) {
         uint32_t x[32];
@@ -464,20 +501,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_rows_kernel(const __g
 // The splits of a tile of rows put together: a thread a row and MERGED entries of the head, neighbouring threads neighbouring rows, 16
 // bytes a store (two portions of 256 rows over 3,000 keys in three: 33 us with the call's other kernels, 59 with 2 bytes a store).
 constexpr int MERGED = 8;
+template <bool MIXED>
 __global__ void __launch_bounds__(ROWS, 6) attention_q8_rows_merge_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
-  const int b = a.request0 + blockIdx.z, piece = blockIdx.x / a.n_kv, kvh = blockIdx.x - piece * a.n_kv, group = a.n_q / a.n_kv;
+  const int piece = blockIdx.x / a.n_kv, kvh = blockIdx.x - piece * a.n_kv, group = a.n_q / a.n_kv;
+  const int b = request_of<MIXED>(a, blockIdx.z, threadIdx.x & 31);
+  if (MIXED && b < 0) return;
   const int qs = a.q_start[b], ql = a.q_start[b + 1] - qs, p0 = a.pos0[b], r = blockIdx.y * ROWS + threadIdx.x;
-  if (ql < a.fewest || (int)blockIdx.y * ROWS >= ql * group ||
-      !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1))
-    return;
-  const int place = many_before(a, b, threadIdx.x & 31);
-  if (place >= a.many || r >= ql * group) return;      // (the first kernel has reported the former)
+  if (ql < a.fewest || r >= ql * group || !within(a, qs, ql, p0, min(min(p0 + ql, a.kv_len[b]), a.max_blocks * a.page_size) - 1)) return;
   float m = -INFINITY, den = 0.f, num[MERGED];
 #pragma unroll
   for (int i = 0; i < MERGED; ++i) num[i] = 0.f;
-  const float* from = part_of(a, place, blockIdx.y, gridDim.y, kvh, 0) + threadIdx.x;
+  const float* from = part_of(a, blockIdx.z, blockIdx.y, gridDim.y, kvh, 0) + threadIdx.x;
   constexpr int STEP = (D + 2) * ROWS;      // to the next split
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, from[s * STEP + D * ROWS]);
@@ -512,6 +548,18 @@ int span_of(int window, int most_keys, int longest) {
   return (int)((keys + KEYS - 1) / KEYS + 1) * KEYS;
 }
 
+template <bool MIXED>
+int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int tiles, cudaStream_t stream) {
+  static LabShared granted;
+  cudaError_t e = lab_allow_shared(granted, (const void*)attention_q8_rows_kernel<MIXED>, SMEM);
+  if (e != cudaSuccess) return (int)e;
+  e = lab_launch(widen_kernel<MIXED>, dim3(a.span / KEYS, a.n_kv, a.many), dim3(WIDEN_THREADS), 0, stream, a);
+  if (e != cudaSuccess) return (int)e;
+  e = lab_launch(attention_q8_rows_kernel<MIXED>, dim3(a.n_kv * a.splits, tiles, a.many), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
+  if (e != cudaSuccess || a.splits == 1) return (int)e;
+  return (int)lab_launch(attention_q8_rows_merge_kernel<MIXED>, dim3(a.n_kv * (D / MERGED), tiles, a.many), dim3(ROWS), 0, stream, a);
+}
+
 }  // namespace
 
 // Bytes of scratch for `many` requests of many rows, whose longest brings `longest` and whose lengths are at most most_keys.
@@ -526,15 +574,16 @@ LAB_EXPORT long long lab_attention_q8_rows_parts(int many, int n_kv, int group, 
 
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, on 16-byte boundaries, out likewise; the `requests` from
 // request0 on, those of `fewest` rows or more (shorter ones are left alone), `many` of them, `longest` the most rows that one
-// brings; lengths are at most most_keys; scratch on a boundary of 16 bytes.  splits: CTAs that share the keys of a
-// tile of rows, their results in `parts` where there are several.  window as lab_first_key takes it.
+// brings; others of that many rows among the requests from look0 up to look1 are reported; lengths are at most most_keys; scratch on a
+// boundary of 16 bytes.  splits: CTAs that share the keys of a tile of rows, their results in `parts` where there are several.  window as
+// lab_first_key takes it.
 struct LabQ8Rows {
   void* out;
   const void *q, *k, *v, *k_scale, *v_scale;
   const int *q_start, *kv_len, *pos0, *block_table;
   void *scratch, *parts;
   long long out_stride, q_stride;
-  int tokens, max_blocks, request0, requests, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys, splits;
+  int tokens, max_blocks, request0, requests, look0, look1, n_q, n_kv, page_size, num_pages, window, fewest, longest, many, most_keys, splits;
   float scale;
 };
 
@@ -544,7 +593,7 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   const long long rows = (long long)c->many * c->n_kv * span;
   if (c->n_kv < 1 || c->n_q < 1 || c->n_q % c->n_kv || c->max_blocks < 1 || c->num_pages < 1 || c->fewest < 1 || c->page_size < 1 || c->request0 < 0 ||
       c->splits < 1 || (c->splits > 1 && (c->parts == nullptr || (((uintptr_t)c->parts) & 3))) || (long long)c->n_kv * c->splits >= (1ll << 31) ||
-      c->most_keys < 1 || rows >= (1ll << 31) || c->requests > 65535 || c->n_kv > 65535 || c->q_stride % 8 || (((uintptr_t)c->q) & 15) ||
+      c->most_keys < 1 || rows >= (1ll << 31) || c->many > c->requests || c->look0 < 0 || c->many > 65535 || c->n_kv > 65535 || c->q_stride % 8 || (((uintptr_t)c->q) & 15) ||
       ((((uintptr_t)c->k) | ((uintptr_t)c->v) | ((uintptr_t)c->scratch)) & 15) || c->scratch == nullptr)
     return (int)cudaErrorInvalidValue;
   Args a;
@@ -552,20 +601,14 @@ LAB_EXPORT int lab_attention_q8_rows(const LabQ8Rows* c, cudaStream_t stream) {
   a.k = (const uint8_t*)c->k, a.v = (const uint8_t*)c->v, a.k_scale = (const uint8_t*)c->k_scale, a.v_scale = (const uint8_t*)c->v_scale;
   a.q_start = c->q_start, a.kv_len = c->kv_len, a.pos0 = c->pos0, a.block_table = c->block_table, a.max_blocks = c->max_blocks;
   a.n_q = c->n_q, a.n_kv = c->n_kv, a.page_size = c->page_size, a.num_pages = c->num_pages, a.window = c->window, a.fewest = c->fewest;
-  a.tokens = c->tokens, a.request0 = c->request0, a.longest = c->longest, a.many = c->many, a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
+  a.tokens = c->tokens, a.request0 = c->request0, a.requests = c->requests, a.look0 = c->look0, a.look1 = c->look1, a.longest = c->longest, a.many = c->many;
+  a.wide_k = (__nv_bfloat16*)c->scratch, a.wide_v = a.wide_k + (size_t)rows * D, a.span = span;
   a.splits = c->splits, a.part = (float*)c->parts, a.scale_log2 = c->scale * LOG2E;
   CUtensorMap mk, mv;
   int rc;
   if ((rc = lab_make_map_bf16(&mk, a.wide_k, rows, D, D, KEYS))) return rc;
   if ((rc = lab_make_map_bf16(&mv, a.wide_v, rows, D, D, KEYS))) return rc;
-  static LabShared granted;
-  cudaError_t e = lab_allow_shared(granted, (const void*)attention_q8_rows_kernel, SMEM);
-  if (e != cudaSuccess) return (int)e;
   const long long tiles = ((long long)c->longest * (c->n_q / c->n_kv) + ROWS - 1) / ROWS;
   if (tiles > 65535) return (int)cudaErrorInvalidValue;
-  e = lab_launch(widen_kernel, dim3(span / KEYS, c->n_kv, c->requests), dim3(WIDEN_THREADS), 0, stream, a);
-  if (e != cudaSuccess) return (int)e;
-  e = lab_launch(attention_q8_rows_kernel, dim3(c->n_kv * c->splits, (unsigned)tiles, c->requests), dim3(THREADS), (size_t)SMEM, stream, mk, mv, a);
-  if (e != cudaSuccess || c->splits == 1) return (int)e;
-  return (int)lab_launch(attention_q8_rows_merge_kernel, dim3(c->n_kv * (D / MERGED), (unsigned)tiles, c->requests), dim3(ROWS), 0, stream, a);
+  return c->many < c->requests ? launch_rows<true>(mk, mv, a, (int)tiles, stream) : launch_rows<false>(mk, mv, a, (int)tiles, stream);
 }

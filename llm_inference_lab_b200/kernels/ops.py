@@ -2365,7 +2365,7 @@ _pack_store = struct.Struct("9P2q9i").pack
 _pack_load = struct.Struct("7Pq5i").pack
 _pack_any = struct.Struct("10P2q10if").pack
 _pack_few = struct.Struct("11P2q14if").pack
-_pack_rows = struct.Struct("12P2q14if").pack
+_pack_rows = struct.Struct("12P2q16if").pack
 _pack_verify = struct.Struct("10P2q4i").pack
 
 
@@ -2594,10 +2594,20 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         scratch = torch.empty((wide + (parts_of(at_once, n_kv, group, longest, splits) if splits > 1 else 0),), dtype=_BYTE, device=q.device)
         room = scratch.data_ptr()
         launch = _entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)
-        for b0, b1, held in _spans_of_many(q_lens, few, at_once) if at_once < len(many) else ((0, n_requests, len(many)),):
+        if at_once < len(many):
+            runs = [(b0, b1, b0, b1, held) for b0, b1, held in _spans_of_many(q_lens, few, at_once)]
+        else:      # from the first to the last of them
+            b0, b1 = 0, n_requests
+            if longest_few:
+                while q_lens[b0] <= few:
+                    b0 += 1
+                while q_lens[b1 - 1] <= few:
+                    b1 -= 1
+            runs = ((b0, b1, 0, n_requests, len(many)),)
+        for b0, b1, look0, look1, held in runs:
             _check(launch(_pack_rows(
-                *tensors, room, room + wide, out.stride(0), stride, tokens, blocks, b0, b1 - b0, n_q, n_kv, page_size, num_pages, window,
-                fewest, longest, held, most_keys, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
+                *tensors, room, room + wide, out.stride(0), stride, tokens, blocks, b0, b1 - b0, look0, look1, n_q, n_kv, page_size,
+                num_pages, window, fewest, longest, held, most_keys, splits, scale), stream), "attention_q8", 2 if splits == 1 else 3)
     if longest_few:
         wide = q8_few_width(longest_few * group)
         if longest_few == 1 and longest == 1:

@@ -116,3 +116,53 @@ def test_requests_shorter_than_told_are_attended(told, rows):
     got = out[: batch.tokens].double().cpu().numpy()
     want, bound = attention(q[: batch.tokens], pages, batch, 4, 2, 64, 0, 0.125, True)
     assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all() and (out[batch.tokens:] == 7.0).all()
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", [
+    [200] + [1] * 40, [1] * 40 + [200], [1] * 35 + [200, 0, 1, 150, 1, 1, 300] + [1] * 33, [150, 200, 5], [1, 130, 130], [0, 130, 0, 2, 0, 140, 0]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_portions_among_many_single_tokens(monkeypatch, splits, rows, d):
+    """First, last, in between and alone: every portion finds its keys, whatever stands beside it."""
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: splits)
+    rng = np.random.default_rng(28)
+    past = [int(p) for p in rng.integers(0, 300, len(rows))]
+    check(rng, rows, past, 4, 2, d, 16)
+    monkeypatch.setattr(ops, "Q8_WIDE_BYTES", 1)
+    check(rng, rows, past, 4, 2, d, 16, window=90)
+
+
+@pytest.mark.parametrize("told, rows, lost", [
+    ([1, 200, 1, 1], [1, 1, 200, 1], 2),            # the portion is another request's, behind the run
+    ([200, 1, 200, 1], [200, 150, 200, 1], 2),      # three in the run where two were told: the last has no place
+    ([1, 200, 1, 200], [150, 200, 1, 1], 0)])       # in front of the run
+def test_portions_where_none_was_told_are_reported(told, rows, lost):
+    rng = np.random.default_rng(29)
+    batch = Batch(rng, rows, [20] * 4, 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 64)
+    q_start, kv_len, pos0, table, *_ = batch.args()
+    q = torch.ones((max(sum(told), batch.tokens), 4 * 64), dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, torch.nan)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, 4, told, 220, 4, 2, 64, 0, 0.125, out=out)
+    with pytest.raises(ops.KernelError, match="row"):
+        ops.take_device_errors()
+    untouched = torch.isnan(out[: batch.tokens])
+    own = untouched[batch.starts[lost]: batch.starts[lost + 1]]
+    assert own.all() and int(untouched.sum()) == own.numel()
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_portions_told_and_not_there(monkeypatch, splits):
+    """Two portions were told; the first has no rows on the device: the second finds its own keys."""
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: splits)
+    rng = np.random.default_rng(30)
+    batch = Batch(rng, [0, 150, 140], [70, 300, 5], 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 64)
+    q_start, kv_len, pos0, table, _, _, most = batch.args()
+    q = torch.from_numpy(rng.standard_normal((600, 4 * 64)).astype(np.float32)).cuda().to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    ops.attention_q8(q, pages, q_start, kv_len, pos0, table, 3, [200, 200, 200], most, 4, 2, 64, 0, 0.125, out=out)
+    ops.take_device_errors()
+    got = out[: batch.tokens].double().cpu().numpy()
+    want, bound = attention(q[: batch.tokens], pages, batch, 4, 2, 64, 0, 0.125, True)
+    assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all() and (out[batch.tokens:] == 7.0).all()
