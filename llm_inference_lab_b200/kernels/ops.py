@@ -2548,9 +2548,10 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     bfloat16 queries of heads of 64 and 128 over pages of 8 to 128 (a power of two) run on the tensor cores; 32-bit queries (in
     32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `Q8_FEW_ROWS` rows
     and query heads of a kv head take scratch for their keys and values in bfloat16, `max_kv_len` of them or what a window leaves,
-    up to `Q8_WIDE_BYTES` at a time.  A request beyond `q_lens`, the rows of q or `max_kv_len` is reported (`take_device_errors`)
-    where a kernel's work is sized by them, and its rows stay as they are; so is one that by its own rows belongs to the kernel for
-    few of them and has more than any that `q_lens` gives that kernel."""
+    and for the results of splits of their keys, up to `Q8_WIDE_BYTES` at a time (or what one request takes).
+
+    A request beyond `q_lens`, the rows of q or `max_kv_len` is reported (`take_device_errors`) where a kernel's work is sized by
+    them, and its rows stay as they are; so is one that by its own rows belongs to the kernel for few of them and has more than any that `q_lens` gives that kernel."""
     k, v, ks, vs = pages
     device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
     shape = q.shape
@@ -2586,12 +2587,12 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
         fewest = few + 1 if longest_few else 1      # (with no call for the others, a request that turns out shorter belongs here too)
         bytes_of, parts_of = _q8_rows_bytes(head_dim)
         many = [n for n in q_lens if n > few]
-        each = bytes_of(1, n_kv, window, most_keys, longest)
-        at_once = max(1, min(len(many), Q8_WIDE_BYTES // each))
         keys = most_keys if window == 0 else min(most_keys, abs(window) + longest)
         splits = q8_rows_splits(n_kv * sum(-(-n * group // 128) for n in many), keys)
+        each, shares = bytes_of(1, n_kv, window, most_keys, longest), parts_of(1, n_kv, group, longest, splits)
+        at_once = max(1, min(len(many), Q8_WIDE_BYTES // (each + shares)))
         wide = at_once * each     # keys and values, then the splits' results (whole tiles of rows: on its boundary)
-        scratch = torch.empty((wide + (parts_of(at_once, n_kv, group, longest, splits) if splits > 1 else 0),), dtype=_BYTE, device=q.device)
+        scratch = torch.empty((wide + at_once * shares,), dtype=_BYTE, device=q.device)
         room = scratch.data_ptr()
         launch = _entry("attention_q8_rows", "lab_attention_q8_rows", head_dim)
         if at_once < len(many):

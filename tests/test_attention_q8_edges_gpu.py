@@ -166,3 +166,25 @@ def test_portions_told_and_not_there(monkeypatch, splits):
     got = out[: batch.tokens].double().cpu().numpy()
     want, bound = attention(q[: batch.tokens], pages, batch, 4, 2, 64, 0, 0.125, True)
     assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all() and (out[batch.tokens:] == 7.0).all()
+
+
+def test_scratch_of_splits_counts_too(monkeypatch):
+    """One long portion beside many short ones: keys, values and the splits' results stay within the bound together."""
+    rng = np.random.default_rng(24)
+    monkeypatch.setattr(ops, "q8_rows_splits", lambda ctas, keys: 2)
+    n_q, d, page = 1, 128, 16
+    batch = Batch(rng, [2048] + [100] * 30, [0] * 31, page)
+    pages = random_pages(ops, rng, batch.num_pages, 1, page, d)
+    x = torch.randn((batch.tokens, n_q * d), device="cuda").to(torch.bfloat16)
+    args = batch.args()
+    together = ops.attention_q8(x, pages, *args, n_q, 1, d, 0, d ** -0.5)
+    # 31 requests of 17 tiles of keys and values, 34.6 MB, with 31 x 16 tiles x 2 splits' results 66 MB more
+    monkeypatch.setattr(ops, "Q8_WIDE_BYTES", 40 << 20)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    apart = ops.attention_q8(x, pages, *args, n_q, 1, d, 0, d ** -0.5)
+    taken = torch.cuda.max_memory_allocated() - before
+    ops.take_device_errors()
+    assert torch.equal(together, apart)
+    assert taken <= (40 << 20) + apart.nbytes + 2 ** 20
