@@ -2551,7 +2551,8 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     and for the results of splits of their keys, up to `Q8_WIDE_BYTES` at a time (or what one request takes).
 
     A request beyond `q_lens`, the rows of q or `max_kv_len` is reported (`take_device_errors`) where a kernel's work is sized by
-    them, and its rows stay as they are; so is one that by its own rows belongs to the kernel for few of them and has more than any that `q_lens` gives that kernel."""
+    them, and its rows stay as they are; so is one that by its own rows belongs to the kernel for few of them and has more than any
+    that `q_lens` gives that kernel."""
     k, v, ks, vs = pages
     device, kind, width, table_shape = q.get_device(), q.dtype, n_q * head_dim, block_table.shape
     shape = q.shape
