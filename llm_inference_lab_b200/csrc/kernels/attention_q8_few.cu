@@ -643,7 +643,31 @@ int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, dim3
   return (int)cudaLaunchKernelEx(&cfg, attention_q8_few_kernel<N>, mk, mv, a);
 }
 
+template <int N>
+int clusters_of(int size) {
+  static LabShared granted;
+  if (lab_allow_shared(granted, (const void*)attention_q8_few_kernel<N>, Layout<N>::SMEM) != cudaSuccess) return -1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Layout<N>::SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, (const void*)attention_q8_few_kernel<N>, &cfg) == cudaSuccess ? n : -1;
+}
+
 }  // namespace
+
+// Clusters of `size` CTAs of a width that the current device holds at once, -1 where it does not say.
+LAB_EXPORT int lab_attention_q8_few_clusters(int width, int size) {
+  if (size < 1 || size > 8) return -1;
+  return width == 16 ? clusters_of<16>(size) : width == 32 ? clusters_of<32>(size) : width == 48 ? clusters_of<48>(size) : -1;
+}
 
 // A call, as the host packs it.  q: `tokens` rows q_stride elements apart, out likewise; requests of up to most_rows rows (longer
 // ones are left alone, and reported where no other call takes them: `alone`), `longest` the most that one of them brings; width: rows a

@@ -2518,13 +2518,45 @@ def q8_few_width(rows: int) -> int:
     return 16 if rows <= 16 else 32 if rows <= 32 else 48
 
 
-def q8_few_splits(ctas: int, width: int, max_kv_len: int) -> int:
-    """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once; up to eight
-    merge inside their cluster, and up to sixteen are not worth a second kernel (16 requests of five drafted tokens over 1,700
-    keys: 13.5 us with eight, 32 with sixteen)."""
-    room = (3 if width <= 16 else 2 if width <= 32 else 1) * sm_count()
-    splits = max(1, min(room // max(1, ctas), -(-max_kv_len // 128)))
-    return 8 if 8 < splits < 16 else splits
+_Q8_HELD = {16: 3, 32: 2, 48: 1}      # CTAs of the few-rows kernel that a multiprocessor holds, by width
+
+
+def q8_few_splits(ctas: int, width: int, max_kv_len: int, places=None) -> int:
+    """CTAs that share the keys of a request, tiles of 128, in the few-rows kernel: as many as the GPU holds at once.  Up to eight
+    merge inside their cluster, for which `places` says how many clusters of a size find room (None: as many as CTAs do): where not
+    all do, those left over run when the others have ended (28 + 4 heads of 128, 4 requests of five tokens over 2,000 keys: 31 us
+    by clusters of seven or eight, of which 15 find room, 17 by six).
+
+    More than eight need a second kernel, which costs the more the more CTAs there are: they have to save a CTA two tiles and a
+    hundredth for each row of all CTAs.  (Single tokens, 7B heads: 1 x 2,000 keys 8.3 us by eight and 9.7 by sixteen, 1 x 4,096
+    9.6 and by thirty-two 8.6, 4 x 4,096 11.4 and 14.5 by twenty-seven, 4 x 8,000 17.1 and 16.3; drafts of five rows 1 x 2,000 15.1
+    and 18.7, 1 x 6,000 21.2 and 19.3, 2 x 8,000 24.5 and 25.2 by eighteen, 2 x 12,000 32.9 and 29.5; 8 x 4,096 single tokens 14.8, 14.5 by
+    twelve and 16.1 by thirteen.)"""
+    tiles = max(1, -(-max_kv_len // 128))
+    splits = max(1, min(_Q8_HELD[width] * sm_count() // max(1, ctas), tiles))
+    merged = min(splits, 8)
+    while merged > 1 and places is not None and places[merged] < ctas:
+        merged -= 1
+    return splits if splits > 8 and tiles * (splits - merged) * 100 >= merged * splits * (200 + ctas * width) else merged
+
+
+def _q8_few_places(device: int, head_dim: int, width: int):
+    """How many clusters of a size (the index, up to eight) of the few-rows kernel the GPU holds.  The runtime's answer is for a CTA a
+    multiprocessor: as many times that as it holds, or, up to nine tenths of all places, as many as clusters on fewer
+    multiprocessors (clusters of eight, two CTAs a multiprocessor: 32 run together, 34 do not; of six, three CTAs: 64, and 72 do
+    not)."""
+    found = _q8_places.get((device, head_dim, width))
+    if found is None:
+        ask = lib("attention_q8_few", {"LAB_HEAD_DIM": head_dim}).lab_attention_q8_few_clusters
+        alone, held = [0] + [int(ask(width, n)) for n in range(1, 9)], _Q8_HELD[width]
+        found = [0] + [max(held * alone[n], min(alone[-(-n // held)], 9 * held * alone[1] // (10 * n))) for n in range(1, 9)]
+        if min(alone[1:]) < 0:
+            raise KernelError("attention_q8: the runtime does not say how many clusters find room")
+        _q8_places[device, head_dim, width] = found
+    return found
+
+
+_q8_places: dict = {}
 
 
 def q8_rows_splits(ctas: int, keys: int) -> int:
@@ -2616,7 +2648,8 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             ctas = n_kv * -(-group // wide) * sum(q_lens)
         else:
             ctas = n_kv * sum(-(-n * group // wide) for n in q_lens if n <= few)
-        splits = q8_few_splits(ctas, wide, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few))
+        splits = q8_few_splits(ctas, wide, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest_few),
+                               _q8_few_places(device, head_dim, wide))
         cluster = 2 <= splits <= 8
         scratch = None
         if splits > 8:
