@@ -2509,8 +2509,17 @@ def _refuse_load(pages, slots, dtype):
 Q8_WIDE_BYTES = 1 << 30
 # Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, by head size.  It takes 48
 # rows a CTA at most and reads the keys again for more (4 requests of 16,000 keys, few- and many-rows kernel: heads of 64, 35 rows 33
-# and 36 us, 49 rows 75 and 36; heads of 128, 84 rows 84 and 88, 112 rows 201 and 89).
+# and 36 us, 49 rows 55 and 35; heads of 128, 84 rows 84 and 88, 112 rows 147 and 89).
 Q8_FEW_ROWS = {64: 48, 128: 96}
+
+
+def q8_few_rows(head_dim: int, requests: int, keys: int) -> int:
+    """`Q8_FEW_ROWS`, and more for a request alone, whose keys in splits fill the GPU either way, without being widened first (1 x 112
+    rows, heads of 128: over 2,000 keys 17 us against 20, 16,000 44 and 48, 60,000 109 and 127; 1 x 84 rows, heads of 64: 15.0 and
+    16.2, 26 and 27, 46 and 72, but 13.7 and 12.0 over 300; 126 rows over 16,000 30.5 and 27.4)."""
+    if requests == 1 and (head_dim == 128 or keys >= 2000):
+        return {64: 96, 128: 128}[head_dim]
+    return Q8_FEW_ROWS[head_dim]
 
 
 def q8_few_width(rows: int) -> int:
@@ -2578,7 +2587,7 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
     counts.  A row that sees no key is 0; rows of no request stay as they are.
 
     bfloat16 queries of heads of 64 and 128 over pages of 8 to 128 (a power of two) run on the tensor cores; 32-bit queries (in
-    32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `Q8_FEW_ROWS` rows
+    32-bit arithmetic), other head sizes up to 256 and other pages on the ordinary units.  Requests of more than `q8_few_rows` rows
     and query heads of a kv head take scratch for their keys and values in bfloat16, `max_kv_len` of them or what a window leaves,
     and for the results of splits of their keys, up to `Q8_WIDE_BYTES` at a time (or what one request takes).
 
@@ -2612,7 +2621,9 @@ def attention_q8(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_l
             BF16 if kind is torch.bfloat16 else F32, scale), stream), "attention_q8")
         return out
     # requests of up to `few` rows, and those of more
-    few = max(1, Q8_FEW_ROWS[head_dim] // group) if stride % 8 == 0 and at % 16 == 0 else longest
+    few = longest
+    if stride % 8 == 0 and at % 16 == 0:
+        few = max(1, q8_few_rows(head_dim, n_requests, max_kv_len if window == 0 else min(max_kv_len, abs(window) + longest)) // group)
     longest_few = longest
     if longest > few:
         longest_few = max((n for n in q_lens if n <= few), default=0)

@@ -32,3 +32,9 @@ def test_clusters_that_find_room(monkeypatch):
 def test_splits_by_what_finds_room_and_pays(monkeypatch, ctas, width, keys, splits):
     monkeypatch.setattr(ops, "sm_count", lambda: 148)
     assert ops.q8_few_splits(ctas, width, keys, places(monkeypatch, width)) == splits
+
+
+@pytest.mark.parametrize("head_dim, requests, keys, rows", [
+    (128, 1, 300, 128), (128, 1, 60000, 128), (128, 2, 300, 96), (128, 40, 16000, 96), (64, 1, 300, 48), (64, 1, 2000, 96), (64, 2, 60000, 48)])
+def test_rows_that_a_request_alone_may_have(head_dim, requests, keys, rows):
+    assert ops.q8_few_rows(head_dim, requests, keys) == rows
