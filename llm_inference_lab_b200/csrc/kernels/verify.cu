@@ -12,8 +12,12 @@
 // very E_t of its row: given that draft and its refusal they are no exponentials any more, and a draw by them favours what the draft
 // passed over.  A call over such drafts says so (`fresh`), and the draw after a refusal then takes a key of its own, the hash of
 // the row's.  (p = (.2, .5, .3), q = (.8, .05, .15), drafts of the sampler: (.2, .542, .258) by the row's key, p by one of its own.)
-// The draw after the last row is the sampler's in either case.  Probabilities are 32-bit: a test or a draw goes another way than in
-// exact arithmetic only where two numbers agree to about 2^-20.
+// The draw after the last row is the sampler's in either case.
+//
+// Probabilities are 32-bit.  p's relative error is about |logit / T| 2^-22 (the quotient's rounding, the largest logit's, and the
+// fast exponential's 2^-22 of its argument) and 2^-20 for the rest; w = p - q keeps that error of p, so w's is p / w times as much.  A
+// test or a draw goes another way than in exact arithmetic only where two numbers agree to that: to 2^-19 with logits of some ten
+// and q away from p.
 //
 // Two launches: the rows' largest entry and sum of exponentials by chunk (every logit read once: the bound, memory), then a
 // cluster of sixteen or four CTAs a request that puts its chunks together, each for itself, decides, and draws over the one row that

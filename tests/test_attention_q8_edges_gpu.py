@@ -188,3 +188,31 @@ def test_scratch_of_splits_counts_too(monkeypatch):
     ops.take_device_errors()
     assert torch.equal(together, apart)
     assert taken <= (40 << 20) + apart.nbytes + 2 ** 20
+
+
+@pytest.mark.parametrize("rows, past, n_q, n_kv, d", [
+    ([1, 1], [300, 4], 100, 2, 64),              # 50 query heads a kv head: two tiles of rows for one token
+    ([1], [3000], 160, 1, 64), ([2, 1], [90, 700], 60, 1, 128), ([1, 1, 1], [10, 0, 150], 130, 1, 128)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_more_rows_than_a_tile_of_the_few_rows_kernel(rows, past, n_q, n_kv, d, window):
+    check(np.random.default_rng(31), rows, past, n_q, n_kv, d, 16, window=window)
+
+
+@pytest.mark.parametrize("rows, past", [([70], [40]), ([33, 5, 1], [0, 600, 90]), ([140, 1], [300, 3])])
+@pytest.mark.parametrize("d, shift", [(64, 2), (64, 4), (128, 6)])
+def test_queries_off_their_boundaries_take_any_number_of_rows(rows, past, d, shift):
+    """Queries 4, 8 or 12 bytes off a boundary of 16 are the few-rows kernel's, however many rows they have."""
+    rng = np.random.default_rng(32)
+    n_q, n_kv, page = 6, 2, 16
+    batch = Batch(rng, rows, past, page)
+    pages = random_pages(ops, rng, batch.num_pages, n_kv, page, d)
+    wide = torch.zeros((batch.tokens, n_q * d + 8), dtype=torch.bfloat16, device="cuda")
+    q = wide[:, shift: shift + n_q * d]
+    q.copy_(torch.from_numpy(rng.standard_normal((batch.tokens, n_q * d)).astype(np.float32)))
+    out = torch.full((batch.tokens, n_q * d + 3), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.attention_q8(q, pages, *batch.args(), n_q, n_kv, d, 0, d ** -0.5, out=out[:, 1: 1 + n_q * d])
+    ops.take_device_errors()
+    assert (out[:, 0] == 7.0).all() and (out[:, 1 + n_q * d:] == 7.0).all()
+    got = out[:, 1: 1 + n_q * d].double().cpu().numpy()
+    want, bound = attention(q, pages, batch, n_q, n_kv, d, 0, d ** -0.5, True)
+    assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all()

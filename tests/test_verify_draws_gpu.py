@@ -107,3 +107,47 @@ def test_an_engines_drafted_step_draws_anew(tmp_path, monkeypatch):
         tokens, counts = (t.tolist() for t in real(*seen["args"], fresh=fresh))
         results.append([tokens[3 * r: 3 * r + counts[r]] for r in range(n)])
     assert told == results[0] != results[1]
+
+
+@pytest.mark.parametrize("offset, temperature", [(0.0, 1.0), (150.0, 0.75), (-300.0, 1.3)])
+def test_replacements_where_the_drafts_probabilities_are_near_the_targets(offset, temperature):
+    """w = p - q cancels: a draw may go to another token than in exact arithmetic only within the error of 32-bit probabilities.
+
+    logit / T has an error of |logit / T| 2^-23 (two roundings), so has the largest one, and the exponential one of 2^-22 of its
+    argument's size; sums, quotients and logarithms a few 2^-23, 2^-20 in all.  p's error reaches w as it is, w's weight by p / w."""
+    from q8_helpers import mix32, mix32_all, uniform
+    rng = np.random.default_rng(10)
+    n, vocab = 200, 4000
+    logits = (rng.standard_normal((2 * n, vocab)) * 2 + offset).astype(np.float32)
+    x = logits.astype(np.float64) / temperature
+    top = x.max(axis=-1, keepdims=True)
+    p = np.exp(x - top)
+    p /= p.sum(axis=-1, keepdims=True)
+    q = (p * (1 + 2.0 ** -9 * rng.standard_normal(p.shape))).astype(np.float32)
+    drafts = np.array([rng.choice(vocab, p=r / r.sum()) for r in p])
+    drafted = np.arange(2 * n), drafts
+    q[drafted] = np.minimum(4 * p[drafted], 0.9)
+    starts, seeds = np.arange(0, 2 * n + 1, 2), np.arange(n)
+    to = lambda a, t: torch.from_numpy(np.ascontiguousarray(a)).to(t).cuda()  # noqa: E731
+    tokens, counts = (t.cpu().numpy() for t in ops.verify_drafts(
+        to(logits, torch.float32), to(drafts, torch.int32), to(starts, torch.int32), to(q, torch.float32),
+        torch.full((n,), temperature, device="cuda"), to(seeds, torch.int32), torch.full((n,), 9, dtype=torch.int32, device="cuda")))
+    ops.take_device_errors()
+    t32 = float(np.float32(temperature))
+    error = (np.abs(x).max() * 2 * 2.0 ** -23 + (top - x) * 2.0 ** -22 + 2.0 ** -20) * p + abs(t32 - temperature) / t32 * (top - x) * p
+    refused = 0
+    for b in range(n):
+        row = 2 * b
+        key = mix32(mix32(b ^ 0x9E3779B9) ^ 9)
+        u, x0 = uniform(mix32(key ^ 0xFFFFFFFF)), drafts[row]
+        if abs(u * q[row, x0] - p[row, x0]) < 1e-3 * p[row, x0]:
+            continue
+        assert (counts[b] == 2) == (u * q[row, x0] < p[row, x0])
+        if counts[b] == 2:
+            continue
+        refused += 1
+        wait = -np.log(uniform(mix32_all(key + np.arange(vocab, dtype=np.uint64) * np.uint64(0x85EBCA6B))))
+        w = np.maximum(p[row] - q[row].astype(np.float64), 0.0)
+        low, high = (w - error[row]) / wait, (w + error[row]) / wait
+        assert high[tokens[row]] * (1 + 2.0 ** -20) >= low.max()
+    assert refused > n // 2
