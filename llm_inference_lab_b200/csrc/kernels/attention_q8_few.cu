@@ -21,10 +21,10 @@
 // over CTAs where there are fewer than the GPU holds, and merged inside a cluster of up to eight or by a second kernel.  Every wait
 // is bounded.
 //
-// Memory bounds the loop (28 + 4 heads of 128, 32 requests of 4,096 keys: 29.2 us, 4.4 TB/s of keys and values, three CTAs a
+// Memory bounds the loop (28 + 4 heads of 128, 32 requests of 4,096 keys: 29.3 us, 4.4 TB/s of keys and values, three CTAs a
 // multiprocessor with a tile of 32 KB each every 3,000 to 4,000 cycles); what is above the bytes is the start, until the queries'
 // codes are there, and the merge: most of a short call (14 + 2 heads of 64, 8 requests of 530 keys: 6.4 us; 16 requests of five
-// drafted tokens over 1,700 keys, 12 + 2 heads of 128: 13.6 us).
+// drafted tokens over 1,700 keys, 12 + 2 heads of 128: 13.5 us).
 #include "quant8_tc.cuh"
 
 #ifndef LAB_HEAD_DIM

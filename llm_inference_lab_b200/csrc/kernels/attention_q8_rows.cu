@@ -19,9 +19,9 @@
 // alone, and none of the ways to shorten them helped: 64 keys a tile, two threads a row, fewer registers.)
 // The groups share a row's reference maximum, to which O is relative: a group decides on it for its tile after the other has
 // for the tile before, which it learns through shared memory.  The reference follows the maximum only when that has grown by
-// more than 2^32 (two portions of 1,024 rows: a tenth less time than with 2^8, where some row of a warp's 32 grows in most of the first tiles;
-// no bit is lost by it, P and O being floating-point numbers), and O is then rescaled in place, the product of the tile before
-// being complete.  Each group keeps a sum of its own.
+// more than 2^32 (two portions of 1,024 rows: a tenth less time than with 2^8, where some row of a warp's 32 grows in most of the
+// first tiles; no bit is lost by it, P and O being floating-point numbers; only values beyond 2^95 or so can take O out of its
+// range), and O is then rescaled in place, the product of the tile before being complete.  Each group keeps a sum of its own.
 //
 // A key that is no number is a row of NaN, and so is one whose value is none (its value then 0): the rows that see it become
 // NaN, and no others.  Rows behind the last key are 0.
@@ -57,7 +57,7 @@ static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 constexpr int TM_S = 0, TM_P = GROUPS * KEYS, TM_O = TM_P + GROUPS * KEYS / 2, TMEM_COLS = 512;
 static_assert(TM_O + D <= TMEM_COLS, "tensor memory holds two S, two P and one O");
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float RESCALE = 32.f;      // P and O have an exponent of eight bits: up to 2^32 too large they are as exact
+constexpr float RESCALE = 32.f;      // P and O have an exponent of eight bits: up to 2^32 too large they are as exact (values below 2^95)
 
 struct Barriers {
   uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[GROUPS], s_empty[GROUPS], p_full[GROUPS],

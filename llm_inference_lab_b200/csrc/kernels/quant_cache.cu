@@ -125,8 +125,8 @@ template <int N> __device__ __forceinline__ void put_codes(uint8_t* to, const fl
 // Whole heads rotated, d a power of two from 16 to 256 (128 for parts: a row's lanes are one warp's), everything on the boundaries
 // of its vectors: d / (2 N) lanes a row, each with N elements of its first half and the N that they turn with.  N = 8 (16 bytes of
 // bfloat16 a load) for rows; N = 2 for parts, whose steps have few rows: four times the lanes then share the sums.  Blocks of 128,
-// ten a multiprocessor (2,048 tokens of 28 + 8 heads of 128: 11.1 us, 12.6 by blocks of 256, four of them; the loads' latency
-// bounds it, 3.3 TB/s).
+// ten a multiprocessor (2,048 tokens of 28 + 8 heads of 128: 11.1 to 11.7 us by what runs around it, 12.1 where that is 11.1 by blocks of
+// 256, four of them; the loads' latency bounds it, 3.2 TB/s).
 template <typename T, bool PARTS, int N>
 __global__ void __launch_bounds__(PARTS ? FEW_THREADS : VEC_THREADS, PARTS ? 1 : 10) store_vec_kernel(const Store s) {
   pdl_trigger();

@@ -2508,8 +2508,8 @@ def _refuse_load(pages, slots, dtype):
 # least), so that many portions beside one long context do not take memory for its length each.
 Q8_WIDE_BYTES = 1 << 30
 # Rows (tokens times query heads of a kv head) up to which a request is attended by the few-rows kernel, by head size.  It takes 48
-# rows a CTA at most and reads the keys again for more (4 requests of 16,000 keys, few- and many-rows kernel: heads of 64, 35 rows 33
-# and 36 us, 49 rows 55 and 35; heads of 128, 84 rows 84 and 88, 112 rows 147 and 89).
+# rows a CTA at most and reads the keys again for more (4 requests of 16,000 keys, few- and many-rows kernel: heads of 64, 35 rows 32
+# and 35 us, 49 rows 55 and 35; heads of 128, 84 rows 82 and 88, 112 rows 147 and 89).
 Q8_FEW_ROWS = {64: 48, 128: 96}
 
 
@@ -2538,9 +2538,9 @@ def q8_few_splits(ctas: int, width: int, max_kv_len: int, places=None) -> int:
 
     More than eight need a second kernel, which costs the more the more CTAs there are: they have to save a CTA two tiles and a
     hundredth for each row of all CTAs.  (Single tokens, 7B heads: 1 x 2,000 keys 8.3 us by eight and 9.7 by sixteen, 1 x 4,096
-    9.6 and by thirty-two 8.6, 4 x 4,096 11.4 and 14.5 by twenty-seven, 4 x 8,000 17.1 and 16.3; drafts of five rows 1 x 2,000 15.1
-    and 18.7, 1 x 6,000 21.2 and 19.3, 2 x 8,000 24.5 and 25.2 by eighteen, 2 x 12,000 32.9 and 29.5; 8 x 4,096 single tokens 14.8, 14.5 by
-    twelve and 16.1 by thirteen.)"""
+    9.6 and by thirty-two 8.6, 4 x 4,096 11.4 and 14.5 by twenty-seven, 4 x 8,000 17.1 and 16.3, 8 x 4,096 14.8, 14.5 by twelve and
+    16.1 by thirteen; drafts of five rows 1 x 2,000 15.1 and 18.7, 1 x 6,000 21.2 and 19.3, 2 x 8,000 24.5 and 25.2 by eighteen, 2 x
+    12,000 32.9 and 29.5.)"""
     tiles = max(1, -(-max_kv_len // 128))
     splits = max(1, min(_Q8_HELD[width] * sm_count() // max(1, ctas), tiles))
     merged = min(splits, 8)

@@ -216,3 +216,25 @@ def test_queries_off_their_boundaries_take_any_number_of_rows(rows, past, d, shi
     got = out[:, 1: 1 + n_q * d].double().cpu().numpy()
     want, bound = attention(q, pages, batch, n_q, n_kv, d, 0, d ** -0.5, True)
     assert (np.abs(got - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all()
+
+
+def test_the_first_call_may_be_a_captured_one(monkeypatch):
+    """How many clusters find room is asked for within a capture too; a replay twice and an eager call leave the same bits."""
+    monkeypatch.setattr(ops, "_q8_places", {})
+    rng = np.random.default_rng(33)
+    batch = Batch(rng, [5, 5, 200, 1], [900, 30, 0, 2000], 16)
+    pages = random_pages(ops, rng, batch.num_pages, 2, 16, 128)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, 14 * 128)).astype(np.float32)).cuda().to(torch.bfloat16)
+    args = batch.args()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attention_q8(q, pages, *args, 14, 2, 128, 0, 128 ** -0.5)
+    assert ops._q8_places and all(n > 0 for found in ops._q8_places.values() for n in found[1:])
+    seen = []
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        seen.append(out.clone())
+    eager = ops.attention_q8(q, pages, *args, 14, 2, 128, 0, 128 ** -0.5)
+    ops.take_device_errors()
+    assert torch.equal(seen[0], seen[1]) and torch.equal(seen[0], eager)
